@@ -192,12 +192,90 @@ __device__ __forceinline__ void tile_coord(int t, const GemmShape& sh, int& tm, 
   }
 }
 
-template <class Cfg, bool B_MN, bool OUT_F32, bool A_MN = false>
+// What a launch fuses to the product (the last kernel parameter).  NoFuse: the plain GEMM.
+enum FuseKind : int {
+  kFuseNone = 0,
+  kFuseXentStats,   // epilogue: per row, maximum and sum of exponentials of the tile's columns; nothing is stored to C
+  kFuseXentGrad,    // epilogue: accumulator -> gradient of the loss with respect to it, before the rounding to bf16
+  kFuseAdd,         // epilogue: FP32 tiles are added to C (one addition per element and launch) instead of stored
+  kFuseLora         // main loop: low-rank K blocks behind the K blocks of A and B, each masked to the rows that use it
+};
+struct NoFuse { static constexpr FuseKind KIND = kFuseNone; };
+struct AddFuse { static constexpr FuseKind KIND = kFuseAdd; };
+
+// Softmax cross entropy, forward.  One pair (maximum, sum of exp(z - maximum)) per row and column
+// tile, at part[column tile * M + row], and the label's logit.  A tile without a finite maximum is kept
+// apart so that the rows' totals come out as log(sum(exp)) says: all -inf -> (-inf, 0), an
+// infinity -> (+inf, +inf), a NaN -> (anything, NaN).
+struct XentStatsFuse {
+  static constexpr FuseKind KIND = kFuseXentStats;
+  float2* part;
+  float* label_logit;       // [M]; written for labels in [0, N)
+  const int64_t* labels;    // [M]
+};
+
+// Per-row numbers of the gradient, laid out by xent_prepare_kernel: d = a * exp(z - lse) - (column == label) * b.
+struct XentRow {
+  float neg_lse_log2e;      // -lse * log2(e)
+  float a, b;
+  int label;                // -1: none
+};
+struct XentGradFuse {
+  static constexpr FuseKind KIND = kFuseXentGrad;
+  const XentRow* rows;      // [M]
+  int col0;                 // vocabulary index of column 0 of this launch
+};
+
+// Low-rank adapters beside the projection:  C[t] += V[t] @ Ad_a,  a = ids[t]  (no term for a < 0).
+// V holds the scaled products with the adapters' first matrices: `terms` bf16 summands of width rp
+// each (rp = the rank rounded up to 16, 32, 64 or 128; columns above the rank are zero).  A row tile runs one
+// set of K steps per distinct id among its rows, in ascending order of the ids, each masked to the TMEM
+// lanes of the rows that have it.  The mask (the instruction's disable-output-lane operand) is what keeps
+// requests apart: an infinity or NaN in one adapter reaches no row of another, as 0 * Inf in a masked
+// operand would.
+struct LoraFuse {
+  static constexpr FuseKind KIND = kFuseLora;
+  CUtensorMap tmV;          // [M, terms * rp], box 64 x 128
+  CUtensorMap tmAd;         // [adapters][R][N], box 64 columns x min(rp, 64) rows; ranks above R read as zero
+  const int32_t* ids;       // [M]
+  int rp, terms;
+};
+
+// The distinct non-negative ids of a row tile, ascending.  Every lane holds the ids of rows
+// lane, 32 + lane, ... of the tile; all lanes of the warp call next() together.
+template <int WORDS>
+struct TileIds {
+  int id[WORDS];
+  int last;
+  __device__ __forceinline__ void load(const int32_t* ids, int row0, int rows, int lane) {
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w) {
+      const int r = row0 + 32 * w + lane;
+      id[w] = r < rows ? ids[r] : -1;
+    }
+    last = -1;
+  }
+  __device__ __forceinline__ int next() {   // -1: no more
+    unsigned best = 0xffffffffu;
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w)
+      if (id[w] > last) best = min(best, (unsigned)id[w]);
+    best = __reduce_min_sync(0xffffffffu, best);
+    if (best == 0xffffffffu) return -1;
+    last = (int)best;
+    return last;
+  }
+};
+
+template <class Cfg, bool B_MN, bool OUT_F32, bool A_MN = false, class Fuse = NoFuse>
 __global__ void __launch_bounds__(Cfg::THREADS, 1)
 gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                  const __grid_constant__ CUtensorMap tmC, void* __restrict__ Cptr, int64_t ldc,
-                 const GemmShape shape, const __grid_constant__ GroupTable groups) {
+                 const GemmShape shape, const __grid_constant__ GroupTable groups, const __grid_constant__ Fuse fuse) {
   constexpr int CG = Cfg::CG, STAGES = Cfg::STAGES, NT = Cfg::NT, ACC_STAGES = Cfg::ACC_STAGES, BN = Cfg::BN;
+  static_assert(Fuse::KIND == kFuseNone || NT == 1, "the fused forms are written for one accumulator per unit");
+  static_assert(Fuse::KIND != kFuseXentGrad || (Cfg::EPI == 1 && !OUT_F32), "the gradient leaves as bf16 through TMA stores");
+  static_assert(Fuse::KIND != kFuseAdd || (Cfg::EPI == 1 && OUT_F32), "tiles are added in FP32 through TMA");
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t sA0 = smem_base;
@@ -359,6 +437,51 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         }
         __syncwarp();
       }
+      if constexpr (Fuse::KIND == kFuseLora) {
+        // one stage per (group of up to 64 / rp adapters, 64 columns of V): the V tile and the adapters' rows
+        const int width = min(fuse.rp, 64), per_stage = 64 / width, passes = (fuse.terms * fuse.rp + 63) / 64;
+        TileIds<4 * CG> tile;
+        tile.load(fuse.ids, tm * CG * kBlockM, shape.M, lane);
+        int slot = 0;
+        bool more = !failed;
+        while (more) {
+          int ad[4], cnt = 0;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) ad[g] = -1;
+          while (more && cnt < per_stage) {
+            const int a = tile.next();
+            if (a < 0) { more = false; break; }
+            if (slot++ % shape.k_splits != split) continue;   // the K ranges of a split share the adapters out
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+              if (g == cnt) ad[g] = a;
+            ++cnt;
+          }
+          if (cnt == 0) break;
+          for (int p = 0; p < passes; ++p, ++it) {
+            const int s = it % STAGES;
+            const uint32_t ph = (it / STAGES) & 1u;
+            if (!mbar_wait_warp(empty_bar(s), ph ^ 1u, kRoleProducer, s)) { failed = true; break; }
+            const uint32_t bar = (CG == 1) ? full_bar(s) : map_to_cta(full_bar(s), 0);
+            if (issuer) {
+              if (cta_rank == 0)
+                mbar_arrive_expect_tx(full_bar(s), CG * (Cfg::A_BYTES + cnt * width * Cfg::BN_CTA * 2));
+              load(sA0 + s * Cfg::A_BYTES, &fuse.tmV, p * 64, m0, 0, bar);
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                if (g < cnt) {
+#pragma unroll
+                  for (int j = 0; j < Cfg::BN_CTA / 64; ++j)
+                    load(sB0 + s * Cfg::B_BYTES + j * 8192 + g * width * 128, &fuse.tmAd,
+                         tn * BN + (int)cta_rank * Cfg::BN_CTA + j * 64, (p * 64) % fuse.rp, ad[g], bar);
+                }
+              }
+            }
+            __syncwarp();
+          }
+          if (failed) break;
+        }
+      }
       if (failed) break;
       if (issuer) trace_stamp(3);
       ++n;
@@ -423,6 +546,57 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           }
           __syncwarp();
         }
+        if constexpr (Fuse::KIND == kFuseLora) {
+          // the K blocks the producer appended, in the same order; A: V tile, K-major; B: adapter rows, N-major
+          constexpr uint32_t ad_idesc = make_idesc_bf16(kBlockM * CG, BN, 0, 1);
+          constexpr uint64_t ad_hi = make_smem_desc_hi(8192, 1024, kLayoutSw128);
+          const int width = min(fuse.rp, 64), per_stage = 64 / width, passes = (fuse.terms * fuse.rp + 63) / 64;
+          int tm, tn, bi, row_base, row_end;
+          decode(t, bi, tm, tn, row_base, row_end);
+          TileIds<4 * CG> tile;
+          tile.load(fuse.ids, tm * CG * kBlockM, shape.M, lane);
+          int slot = 0;
+          bool more = !failed;
+          while (more) {
+            int ad[4], cnt = 0;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) ad[g] = -1;
+            while (more && cnt < per_stage) {
+              const int a = tile.next();
+              if (a < 0) { more = false; break; }
+              if (slot++ % shape.k_splits != split) continue;
+#pragma unroll
+              for (int g = 0; g < 4; ++g)
+                if (g == cnt) ad[g] = a;
+              ++cnt;
+            }
+            if (cnt == 0) break;
+            for (int p = 0; p < passes; ++p, ++it) {
+              const int s = it % STAGES;
+              const uint32_t ph = (it / STAGES) & 1u;
+              if (!mbar_wait_warp(full_bar(s), ph, kRoleMma, s)) { failed = true; break; }
+              tc_fence_after_sync();
+              const int terms_here = min(per_stage, (fuse.terms * fuse.rp - p * 64) / width);   // summands (or parts of one) in this V tile
+#pragma unroll
+              for (int g = 0; g < 4; ++g) {
+                if (g < cnt) {
+                  uint32_t off[4 * CG];   // set bits: TMEM lanes (rows) left as they are
+#pragma unroll
+                  for (int w = 0; w < 4 * CG; ++w) off[w] = ~__ballot_sync(0xffffffffu, tile.id[w] == ad[g]);
+                  if (issuer) {
+                    for (int q = 0; q < terms_here; ++q)
+                      for (int k = 0; k < width / kUmmaK; ++k)
+                        mma_f16_masked<CG>(d_tmem, smem_desc(make_smem_desc_hi(16, 1024, kLayoutSw128), sA0 + s * Cfg::A_BYTES + (q * width + k * kUmmaK) * 2),
+                                           smem_desc(ad_hi, sB0 + s * Cfg::B_BYTES + (g * width + k * kUmmaK) * 128), ad_idesc, off);
+                  }
+                }
+              }
+              if (issuer) commit(empty_bar(s));
+              __syncwarp();
+            }
+            if (failed) break;
+          }
+        }
         if (failed) break;
         if (issuer) { trace_stamp(5); commit(tfull_bar(acc)); }   // accumulator complete -> epilogue warps of both CTAs
         __syncwarp();
@@ -460,7 +634,51 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       bool released = false;   // TMEM already handed back inside the branch below
       const int row = m0 + lane;
 
-      if constexpr (Cfg::EPI == 0) {
+      if constexpr (Fuse::KIND == kFuseXentStats) {
+        // One row per lane; the running maximum and sum of a softmax over the tile, 32 columns at a time.
+        constexpr float kLog2e = 1.4426950408889634f;
+        const int64_t label64 = row < row_end ? fuse.labels[row] : -1;
+        const int label = (label64 >= n0 && label64 < (int64_t)n0 + BN && label64 < shape.N) ? (int)label64 : -1;
+        float top = -INFINITY, sum = 0.f, hit = 0.f;
+#pragma unroll 1
+        for (int c = 0; c < BN / 32; ++c) {
+          const int col = n0 + c * 32;
+          if (col >= shape.N) break;
+          uint32_t v[32];
+          tmem_ld_32x32b_x32(t_addr + c * 32, v);
+          tmem_ld_wait();
+          if (col + 32 > shape.N) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (col + j >= shape.N) v[j] = 0xff800000u;   // -inf: no column
+          }
+          float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int j = 0; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(v[j]));
+          const float now = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+          const float base = isinf(now) ? 0.f : now;       // exp(-inf - 0) = 0, exp(inf - 0) = inf: no NaN of our making
+          const float nb = -base * kLog2e;
+          sum = sum * (isinf(top) ? 1.f : exp2_approx(fmaf(top, kLog2e, nb)));   // top = -inf: the sum is 0 or NaN
+          float part[4] = {sum, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int j = 0; j < 32; ++j) part[j & 3] += exp2_approx(fmaf(__uint_as_float(v[j]), kLog2e, nb));
+          sum = (part[0] + part[1]) + (part[2] + part[3]);
+          top = now;
+          if (label >= col && label < col + 32) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+              if (col + j == label) hit = __uint_as_float(v[j]);
+          }
+        }
+        if (row < row_end) {
+          const long long n_part = (long long)shape.tiles_n * shape.M;
+          (void)n_part;
+          float2* dst = fuse.part + (int64_t)tn * shape.M + row;
+          if (GEMM_B200_IN_BOUNDS(dst, fuse.part, n_part * 8, 8, 40)) *dst = make_float2(top, sum);
+          if (label >= 0 && GEMM_B200_IN_BOUNDS(fuse.label_logit + row, fuse.label_logit, (long long)shape.M * 4, 4, 41))
+            fuse.label_logit[row] = hit;
+        }
+      } else if constexpr (Cfg::EPI == 0) {
 #pragma unroll 1
         for (int c = 0; c < BN / 32; ++c) {
           uint32_t v[32];
@@ -542,6 +760,11 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       } else {
         // 128-byte-wide column slabs: 64 bf16 or 32 f32 columns per TMA store of 32 rows.
         constexpr int SLAB_COLS = OUT_F32 ? 32 : 64;
+        XentRow xr = {0.f, 0.f, 0.f, -1};
+        if constexpr (Fuse::KIND == kFuseXentGrad) {
+          if (row < row_end) xr = fuse.rows[row];
+        }
+        (void)xr;
 #pragma unroll 1
         for (int c = 0; c < BN / SLAB_COLS; ++c, ++store_it) {
           const uint32_t buf = stage0 + (store_it % Cfg::EPI_BUFS) * Cfg::EPI_WARP_BUF;
@@ -564,6 +787,21 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
               uint32_t v[32];
               tmem_ld_32x32b_x32(t_addr + c * 64 + h * 32, v);
               tmem_ld_wait();
+              if constexpr (Fuse::KIND == kFuseXentGrad) {
+                // a row without weight gets exact zeros, whatever its logits are
+                const bool live = xr.a != 0.f || xr.b != 0.f;
+                const int at = xr.label - (fuse.col0 + n0 + c * 64 + h * 32);
+#pragma unroll
+                for (int j = 0; j < 32; ++j) {
+                  const float p = exp2_approx(fmaf(__uint_as_float(v[j]), 1.4426950408889634f, xr.neg_lse_log2e));
+                  v[j] = live ? __float_as_uint(xr.a * p) : 0u;
+                }
+                if (at >= 0 && at < 32) {
+#pragma unroll
+                  for (int j = 0; j < 32; ++j)
+                    if (j == at) v[j] = __float_as_uint(__uint_as_float(v[j]) - xr.b);
+                }
+              }
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 uint32_t p[4];
@@ -583,7 +821,9 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           __syncwarp();
           const int x = n0 + c * SLAB_COLS;
           if (lane == 0) {
-            if (m0 < shape.M && x < shape.N) tma_store_3d(&tmC, x, m0, shape.k_splits > 1 ? split : bi, buf);   // split-K: slice `split` of the scratch
+            if constexpr (Fuse::KIND == kFuseAdd) {
+              if (m0 < shape.M && x < shape.N) tma_add_f32_3d(&tmC, x, m0, shape.k_splits > 1 ? split : bi, buf);
+            } else if (m0 < shape.M && x < shape.N) tma_store_3d(&tmC, x, m0, shape.k_splits > 1 ? split : bi, buf);   // split-K: slice `split` of the scratch
             tma_store_commit();
           }
         }

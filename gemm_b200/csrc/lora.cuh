@@ -1,0 +1,453 @@
+// Low-rank adapters of many requests, the passes beside the shared projection.
+//
+//   y_t = x_t W + s_a (x_t A_a^T) B_a,   a = ids[t]        A [n, R, D], B [n, R, N]
+//   dA_a = s_a sum_{t: ids[t] = a} (dy_t B_a^T)^T x_t,     dB_a = s_a sum_{t: ids[t] = a} (x_t A_a^T)^T dy_t
+//
+// The projection with its second factor is one launch of the GEMM kernel (LoraFuse in gemm_bf16.cuh); here are
+// the products with the first factor (V = s x A^T, and dy B^T for the gradient) and the sums over a
+// request's tokens.  Both read their long operand once and do little arithmetic on it, so they use
+// mma.sync from registers: what bounds them is the read.
+//
+// The reference has no counterpart; the products extend its operator (naive/naive.cpp:6-22).
+#pragma once
+#include "common.cuh"
+#include "tc_common.cuh"
+#include "gemm_bf16.cuh"
+
+namespace gemm_b200 {
+namespace tc {
+
+__device__ __forceinline__ void mma_m16n8k16_bf16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                                  uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ uint4 ldg_16(const void* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
+__device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
+  return v;
+}
+
+// ---------------------------------------------------------------------------------------
+// V[t, r] = s_a sum_k X[t, k] A_a[r, k], a = ids[t], as `terms` bf16 summands of width rp side by side
+// (three of them carry 24 bits for FP32 results; one is the ordinary rounding for bf16 results, of the size of
+// the rounding of the result).  Rows without an adapter are not written (nothing reads them); a row
+// with an id >= n becomes NaN.
+//
+// One block: up to 16 * MT rows and, in a cluster of gridDim.y blocks, a share of K.  Its eight warps are
+// dealt out to the distinct adapters of the rows first and to K second, so that a block of one
+// request and a block of sixteen keep the same number of loads in flight.  A warp loads its fragments
+// straight from global memory, 16 bytes per lane: the order of k inside a product is free, so a lane's eight consecutive k
+// become the k pairs of two MMAs in the same way for X and A.  A row is loaded only under its
+// own adapter.  Every warp leaves its rows' sums in a buffer of its own; the final pass adds them over
+// the warps and the cluster in a fixed order.
+// ---------------------------------------------------------------------------------------
+struct ShrinkProblem {
+  const __nv_bfloat16* X;
+  const __nv_bfloat16* A;
+  __nv_bfloat16* V;
+  int64_t ldx, lda, stride_a;
+  int K;
+};
+struct ShrinkArgs {
+  ShrinkProblem p[2];
+  const int32_t* ids;
+  const float* scales;   // may be null: 1
+  int T, R, n, rp, terms, rows_per_block, chunks;   // chunks of 64 ranks
+};
+constexpr int kShrinkWarps = 8;
+
+template <int MT, int NT8>
+struct ShrinkShape {
+  static constexpr int ROWS = 16 * MT, COLS = 8 * NT8, LD = COLS + 8;
+  static constexpr int SMEM_BYTES = kShrinkWarps * ROWS * LD * 4;
+  static constexpr int UNROLL = (2 * MT + NT8 <= 6) ? 4 : 2;
+};
+
+template <int MT, int NT8>
+__global__ void __launch_bounds__(32 * kShrinkWarps)
+lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
+  using S = ShrinkShape<MT, NT8>;
+  constexpr int WORDS = (S::ROWS + 31) / 32, U = S::UNROLL;
+  extern __shared__ float shrink_buf[];   // [warp][row][LD]
+  __shared__ int slot_of[S::ROWS];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int rank = blockIdx.y, ranks = gridDim.y;
+  const int chunk = blockIdx.z % args.chunks;
+  const ShrinkProblem& pr = args.p[blockIdx.z / args.chunks];
+  const int row0 = blockIdx.x * args.rows_per_block;
+  const int row_end = min(args.T, row0 + args.rows_per_block);
+  pdl_wait();
+  pdl_launch_dependents();
+
+  TileIds<WORDS> ids;
+  ids.load(args.ids, row0, row_end, lane);
+  int slots = 0;
+  while (ids.next() >= 0) ++slots;
+  ids.last = -1;
+  const int by_slot = slots > 4 ? 8 : slots > 2 ? 4 : slots > 1 ? 2 : 1;
+  const int by_k = kShrinkWarps / by_slot;
+  const int my_slot = warp % by_slot, my_k = rank * by_k + warp / by_slot, k_stride = ranks * by_k;
+  const int steps = (pr.K + 31) / 32;
+
+  for (int slot = 0; slot < slots; ++slot) {
+    const int a = ids.next();
+    if (slot % by_slot != my_slot) continue;
+    // which of this lane's rows have the adapter
+    bool mine[MT][2];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int lr = mt * 16 + h * 8 + g;
+        mine[mt][h] = __shfl_sync(0xffffffffu, ids.id[(mt * 16 + h * 8) / 32], lr % 32) == a;
+      }
+    float acc[MT][NT8][4];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT8; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[mt][nt][e] = a < args.n ? 0.f : NAN;
+    if (a < args.n) {
+      const __nv_bfloat16* xp[MT][2];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) xp[mt][h] = pr.X + (int64_t)(row0 + mt * 16 + h * 8 + g) * pr.ldx + q * 8;
+      const __nv_bfloat16* ap = pr.A + (int64_t)a * pr.stride_a + (int64_t)(chunk * 64 + g) * pr.lda + q * 8;
+      const int ranks_left = args.R - chunk * 64 - g;
+      for (int s0 = my_k; s0 < steps; s0 += U * k_stride) {
+        uint4 x[U][MT][2], w[U][NT8];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          const int k = (s0 + u * k_stride) * 32;
+          const bool in = k + q * 8 < pr.K;
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) x[u][mt][h] = in && mine[mt][h] ? ldg_16(xp[mt][h] + k) : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+          for (int nt = 0; nt < NT8; ++nt)
+            w[u][nt] = in && nt * 8 < ranks_left ? ldg_16(ap + (int64_t)(nt * 8) * pr.lda + k) : make_uint4(0u, 0u, 0u, 0u);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+            for (int nt = 0; nt < NT8; ++nt) {
+              mma_m16n8k16_bf16(acc[mt][nt], x[u][mt][0].x, x[u][mt][1].x, x[u][mt][0].y, x[u][mt][1].y, w[u][nt].x, w[u][nt].y);
+              mma_m16n8k16_bf16(acc[mt][nt], x[u][mt][0].z, x[u][mt][1].z, x[u][mt][0].w, x[u][mt][1].w, w[u][nt].z, w[u][nt].w);
+            }
+      }
+    }
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int lr = mt * 16 + h * 8 + g;
+        if (mine[mt][h]) {
+          if (q == 0) slot_of[lr] = slot;   // the same value from every warp that writes it
+          float* dst = shrink_buf + (warp * S::ROWS + lr) * S::LD + 2 * q;
+#pragma unroll
+          for (int nt = 0; nt < NT8; ++nt)
+            *reinterpret_cast<float2*>(dst + nt * 8) = make_float2(acc[mt][nt][2 * h], acc[mt][nt][2 * h + 1]);
+        }
+      }
+  }
+  __syncthreads();
+  if (ranks > 1) {
+    cluster_arrive();
+    cluster_wait();
+  }
+  const int64_t ldv = (int64_t)args.terms * args.rp;
+  const uint32_t base = smem_u32(shrink_buf);
+  for (int e = rank * 32 * kShrinkWarps + threadIdx.x; e < (row_end - row0) * S::COLS; e += ranks * 32 * kShrinkWarps) {
+    const int lr = e / S::COLS, c = e % S::COLS, r = chunk * 64 + c;
+    const int a = args.ids[row0 + lr];
+    if (a < 0) continue;
+    float sum = 0.f;
+    const int w0 = slot_of[lr] % by_slot;
+    for (int b = 0; b < ranks; ++b) {
+      if (ranks > 1) {
+        const uint32_t remote = map_to_cta(base, (uint32_t)b);
+        for (int w = w0; w < kShrinkWarps; w += by_slot) sum += ld_shared_cluster_f32(remote + 4u * (uint32_t)((w * S::ROWS + lr) * S::LD + c));
+      } else {
+        for (int w = w0; w < kShrinkWarps; w += by_slot) sum += shrink_buf[(w * S::ROWS + lr) * S::LD + c];
+      }
+    }
+    float v = r < args.R ? sum : 0.f;
+    if (a < args.n && r < args.R && args.scales) v *= args.scales[a];
+    __nv_bfloat16* dst = pr.V + (row0 + lr) * ldv + r;
+    const long long v_bytes = (long long)args.T * ldv * 2;
+    (void)v_bytes;
+    for (int t = 0; t < args.terms; ++t) {
+      const __nv_bfloat16 h = __float2bfloat16_rn(v);
+      if (GEMM_B200_IN_BOUNDS(dst + t * args.rp, pr.V, v_bytes, 2, 50)) dst[t * args.rp] = h;
+      const float back = __bfloat162float(h);
+      v = isinf(back) ? 0.f : v - back;   // an infinity is whole in its first summand
+    }
+  }
+  __syncwarp();
+  if (ranks > 1) {   // no block leaves while another one reads its sums
+    cluster_arrive();
+    cluster_wait();
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// Tokens by adapter, for the gradient: perm[start[a], start[a + 1]) are the rows with id a, ascending.
+// One block per adapter scans the ids twice (counts, then places): no atomics, one possible result.
+// ---------------------------------------------------------------------------------------
+__global__ void __launch_bounds__(1024)
+lora_sort_kernel(const int32_t* __restrict__ ids, int T, int n, int32_t* __restrict__ perm, int32_t* __restrict__ start) {
+  __shared__ int eq[32], lt[32];
+  const int a = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int per = (T + 1023) / 1024 * 32;   // rows per warp, a multiple of 32
+  const int r0 = min(T, warp * per), r1 = min(T, r0 + per);
+  int n_eq = 0, n_lt = 0;
+#pragma unroll 8
+  for (int r = r0; r < r1; r += 32) {
+    const int id = r + lane < r1 ? ids[r + lane] : -1;
+    n_eq += __popc(__ballot_sync(0xffffffffu, id == a));
+    n_lt += __popc(__ballot_sync(0xffffffffu, id >= 0 && id < a));
+  }
+  if (lane == 0) { eq[warp] = n_eq; lt[warp] = n_lt; }
+  __syncthreads();
+  int at = 0, before = 0, all = 0;
+  for (int w = 0; w < 32; ++w) {
+    at += lt[w];
+    all += eq[w];
+    if (w < warp) before += eq[w];
+  }
+  if (threadIdx.x == 0) {
+    start[a] = at;
+    if (a == n - 1) start[n] = at + all;
+  }
+  if (all == 0) return;
+  at += before;
+  for (int r = r0; r < r1; r += 32) {
+    const int id = r + lane < r1 ? ids[r + lane] : -1;
+    const unsigned hit = __ballot_sync(0xffffffffu, id == a);
+    if (id == a) perm[at + __popc(hit & ((1u << lane) - 1u))] = r + lane;
+    at += __popc(hit);
+  }
+}
+
+// ---------------------------------------------------------------------------------------
+// G_a[r, c] = sum over the tokens of a of P[t, r] Q[t, c]: dA from P = s dy B^T and Q = x, dB from P = s x A^T and Q = dy.
+//
+// The token axis, sorted by adapter, is cut into blocks of equal length whatever the requests' shares are (one
+// adapter with every token, or sixty with a few each); a block owns 128 columns and walks the adapters that
+// its range touches, 32 tokens per step, the loads running ahead across the adapters' borders.
+// A sum that lies inside one block goes straight to the result; the others leave a partial sum at slot
+// (block + adapter), which no other pair shares because both only grow along the axis, and
+// lora_join_kernel adds them in the order of the blocks.  Rows are gathered, so only a request's own tokens
+// are ever multiplied: nothing of one request reaches another's gradient.
+// ---------------------------------------------------------------------------------------
+struct GradProblem {
+  const __nv_bfloat16* P;   // [T, terms * rp]
+  const __nv_bfloat16* Q;   // [T, cols], pitch ldq
+  void* out;                // [n, R, cols]
+  float* part;              // [blocks + n][R][cols]
+  int64_t ldq;
+  int cols, first_chunk;    // column chunks [first_chunk, ...) of the grid belong to this problem
+};
+struct GradArgs {
+  GradProblem p[2];
+  const int32_t* perm;
+  const int32_t* start;
+  int n, R, block_tokens;
+};
+constexpr int kGradCols = 128, kGradTokens = 32, kGradStages = 4, kGradThreads = 128;
+
+template <int MT, int TERMS>
+struct GradShape {
+  static constexpr int RP = 16 * MT;
+  static constexpr int Q_PITCH = kGradCols * 2 + 16, P_PITCH = RP * TERMS * 2 + 16;   // odd multiples of 16 bytes: ldmatrix without conflicts
+  static constexpr int STAGE_BYTES = kGradTokens * (Q_PITCH + P_PITCH);
+  static constexpr int SMEM_BYTES = kGradStages * STAGE_BYTES;
+};
+
+// Walks the steps of one block: positions [pos, end) of adapter a, at most 32 at a time.
+struct GradWalk {
+  int a, pos, end, limit;
+  __device__ __forceinline__ void settle(const int32_t* start, int n) {   // skip adapters that are used up
+    while (a < n && pos >= end) {
+      ++a;
+      if (a < n) end = min(limit, start[a + 1]);
+    }
+    if (pos >= limit) a = n;
+  }
+};
+
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool in) {
+  const int bytes = in ? 16 : 0;   // 0: sixteen zero bytes, nothing is read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+template <int MT, int TERMS, bool OUT_F32>
+__global__ void __launch_bounds__(kGradThreads)
+lora_grad_kernel(const __grid_constant__ GradArgs args) {
+  using S = GradShape<MT, TERMS>;
+  extern __shared__ __align__(16) uint8_t grad_smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const GradProblem& pr = args.p[(int)blockIdx.x >= args.p[1].first_chunk ? 1 : 0];
+  const int c0 = ((int)blockIdx.x - pr.first_chunk) * kGradCols;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int total = args.start[args.n];
+  const int lo = blockIdx.y * args.block_tokens, hi = min(total, lo + args.block_tokens);
+  if (lo >= hi) return;
+  // the adapter that position `lo` belongs to: the last one that starts at or before it
+  int a0 = 0, a1 = args.n - 1;
+  while (a0 < a1) {
+    const int mid = (a0 + a1 + 1) >> 1;
+    if (args.start[mid] <= lo) a0 = mid; else a1 = mid - 1;
+  }
+  GradWalk ld{a0, lo, min(hi, args.start[a0 + 1]), hi};
+  ld.settle(args.start, args.n);
+  GradWalk cu = ld;
+
+  const uint32_t smem = smem_u32(grad_smem);
+  const int64_t ldp = (int64_t)S::RP * TERMS;
+  auto load_step = [&](int stage) {   // the next step of `ld` into a stage; an empty group once it is through
+    if (ld.a < args.n) {
+      const int cnt = min(kGradTokens, ld.end - ld.pos);
+      const uint32_t qs = smem + stage * S::STAGE_BYTES, ps = qs + kGradTokens * S::Q_PITCH;
+#pragma unroll
+      for (int i = 0; i < kGradTokens * (kGradCols / 8) / kGradThreads; ++i) {
+        const int e = threadIdx.x + i * kGradThreads, t = e / (kGradCols / 8), c = e % (kGradCols / 8) * 8;
+        const bool in = t < cnt && c0 + c < pr.cols;
+        const __nv_bfloat16* src = pr.Q;
+        if (in) src += (int64_t)args.perm[ld.pos + t] * pr.ldq + c0 + c;
+        cp_async_16(qs + t * S::Q_PITCH + c * 2, src, in);
+      }
+      constexpr int PV = S::RP * TERMS / 8;
+      for (int e = threadIdx.x; e < kGradTokens * PV; e += kGradThreads) {
+        const int t = e / PV, c = e % PV * 8;
+        const bool in = t < cnt;
+        const __nv_bfloat16* src = pr.P;
+        if (in) src += (int64_t)args.perm[ld.pos + t] * ldp + c;
+        cp_async_16(ps + t * S::P_PITCH + c * 2, src, in);
+      }
+      ld.pos += cnt;
+      ld.settle(args.start, args.n);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int s = 0; s < kGradStages - 1; ++s) load_step(s);
+
+  float acc[MT][4][4];
+  auto clear = [&] {
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[mt][nt][e] = 0.f;
+  };
+  clear();
+  const int warp_c = warp * 32;
+  for (int it = 0; cu.a < args.n; ++it) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kGradStages - 2) : "memory");
+    __syncthreads();
+    load_step((it + kGradStages - 1) % kGradStages);   // into the stage every warp finished with before the barrier
+    const uint32_t qs = smem + (it % kGradStages) * S::STAGE_BYTES, ps = qs + kGradTokens * S::Q_PITCH;
+#pragma unroll
+    for (int k = 0; k < kGradTokens / 16; ++k) {
+      uint32_t b[2][4];   // 16 tokens x 32 columns
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        ldmatrix_x4_trans(b[h], qs + (k * 16 + (lane & 15)) * S::Q_PITCH + (warp_c + h * 16 + (lane >> 4) * 8) * 2);
+#pragma unroll
+      for (int t = 0; t < TERMS; ++t)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          uint32_t r[4];    // P^T: 16 ranks x 16 tokens; matrices (tokens 0-7, 8-15) x (ranks 0-7, 8-15)
+          ldmatrix_x4_trans(r, ps + (k * 16 + (lane >> 4) * 8 + (lane & 7)) * S::P_PITCH + (t * S::RP + mt * 16 + ((lane >> 3) & 1) * 8) * 2);
+#pragma unroll
+          for (int nt = 0; nt < 4; ++nt)
+            mma_m16n8k16_bf16(acc[mt][nt], r[0], r[1], r[2], r[3], b[nt >> 1][(nt & 1) * 2], b[nt >> 1][(nt & 1) * 2 + 1]);
+        }
+    }
+    cu.pos += min(kGradTokens, cu.end - cu.pos);
+    if (cu.pos >= cu.end) {   // the adapter's share of this block is complete
+      const int a = cu.a;
+      const bool whole = args.start[a] >= lo && args.start[a + 1] <= hi;
+      const long long out_elems = (long long)args.n * args.R * pr.cols;
+      (void)out_elems;
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = mt * 16 + h * 8 + g;
+          if (r >= args.R) continue;
+#pragma unroll
+          for (int nt = 0; nt < 4; ++nt) {
+            const int c = c0 + warp_c + nt * 8 + 2 * q;
+            if (c >= pr.cols) continue;
+            const float x = acc[mt][nt][2 * h], y = acc[mt][nt][2 * h + 1];
+            if (!whole) {
+              *reinterpret_cast<float2*>(pr.part + ((int64_t)(blockIdx.y + a) * args.R + r) * pr.cols + c) = make_float2(x, y);
+            } else {
+              const int64_t at = ((int64_t)a * args.R + r) * pr.cols + c;
+              if (!GEMM_B200_IN_BOUNDS(static_cast<char*>(pr.out) + at * (OUT_F32 ? 4 : 2), pr.out, out_elems * (OUT_F32 ? 4 : 2), OUT_F32 ? 8 : 4, 51)) continue;
+              if constexpr (OUT_F32) *reinterpret_cast<float2*>(static_cast<float*>(pr.out) + at) = make_float2(x, y);
+              else *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(pr.out) + at) = __floats2bfloat162_rn(x, y);
+            }
+          }
+        }
+      clear();
+      cu.settle(args.start, args.n);
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// Sums the partial sums of adapters whose tokens span blocks, in the order of the blocks, and zeroes the
+// gradients of adapters without a token.
+template <bool OUT_F32>
+__global__ void __launch_bounds__(256)
+lora_join_kernel(const __grid_constant__ GradArgs args) {
+  const int a = blockIdx.y;
+  const GradProblem& pr = args.p[blockIdx.z];
+  pdl_wait();
+  pdl_launch_dependents();
+  const int s0 = args.start[a], s1 = args.start[a + 1];
+  const int b0 = s0 / args.block_tokens, b1 = (s1 - 1) / args.block_tokens;
+  if (s1 > s0 && b0 == b1) return;
+  const int64_t elems = (int64_t)args.R * pr.cols;   // a multiple of 8
+  for (int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; e < elems; e += (int64_t)gridDim.x * 1024) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (s1 > s0) {
+#pragma unroll 4
+      for (int b = b0; b <= b1; ++b) {
+        const float4 v = *reinterpret_cast<const float4*>(pr.part + (int64_t)(b + a) * elems + e);
+        acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+      }
+    }
+    const int64_t at = (int64_t)a * elems + e;
+    if constexpr (OUT_F32) {
+      *reinterpret_cast<float4*>(static_cast<float*>(pr.out) + at) = acc;
+    } else {
+      __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x, acc.y), hi = __floats2bfloat162_rn(acc.z, acc.w);
+      *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(pr.out) + at) =
+          make_uint2(*reinterpret_cast<uint32_t*>(&lo), *reinterpret_cast<uint32_t*>(&hi));
+    }
+  }
+}
+
+}  // namespace tc
+}  // namespace gemm_b200

@@ -59,6 +59,13 @@ __device__ __forceinline__ void trace_stamp(int slot) {
 __device__ __forceinline__ void trace_stamp(int) {}
 #endif
 
+// 2^x by the hardware's approximation (relative error 2^-22 or so; subnormal results flush to zero)
+__device__ __forceinline__ float exp2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
   return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }
@@ -311,6 +318,12 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* map, int x, int 
                ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(x), "r"(y), "r"(z)
                : "memory");
 }
+// adds the FP32 tile in shared memory to global memory, element by element
+__device__ __forceinline__ void tma_add_f32_3d(const CUtensorMap* map, int x, int y, int z, uint32_t src) {
+  asm volatile("cp.reduce.async.bulk.tensor.3d.global.shared::cta.add.tile.bulk_group [%0, {%2, %3, %4}], [%1];"
+               ::"l"(reinterpret_cast<uint64_t>(map)), "r"(src), "r"(x), "r"(y), "r"(z)
+               : "memory");
+}
 __device__ __forceinline__ void tma_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void tma_store_wait_read() {
@@ -370,6 +383,26 @@ __device__ __forceinline__ void mma_f16(uint32_t d_tmem, uint64_t adesc, uint64_
         "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
         "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n"
         ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// D[tmem] += A * B for the TMEM lanes (rows of the tile) whose bit in `off` is clear; the other lanes keep their
+// values whatever A holds there.  Word w covers rows [32 w, 32 w + 32) of the tile (of both CTAs of a pair).
+template <int CG>
+__device__ __forceinline__ void mma_f16_masked(uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
+                                               const uint32_t (&off)[4 * CG]) {
+  if constexpr (CG == 1)
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.eq.u32 p, 0, 0;\n"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7}, p;\n}\n"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3])
+        : "memory");
+  else
+    asm volatile(
+        "{\n.reg .pred p;\nsetp.eq.u32 p, 0, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%4, %5, %6, %7, %8, %9, %10, %11}, p;\n}\n"
+        ::"r"(d_tmem), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(off[0]), "r"(off[1]), "r"(off[2]), "r"(off[3]),
+        "r"(off[4]), "r"(off[5]), "r"(off[6]), "r"(off[7])
         : "memory");
 }
 

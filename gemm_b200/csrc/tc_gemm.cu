@@ -7,6 +7,8 @@
 
 #include "gemm_bf16.cuh"
 #include "gemm_bf16_ksplit.cuh"
+#include "xent.cuh"
+#include "lora.cuh"
 #include "gemm_mxfp8.cuh"
 #include "gemm_mxfp8_ksplit.cuh"
 
@@ -362,9 +364,10 @@ struct Bf16Args {
   int k_splits = 1;
 };
 
-// One instantiation per (config, B layout, output type); A_MN: A is stored transposed, [K, M] row-major.
-template <class Cfg, bool B_MN, bool OUT_F32, bool A_MN = false>
-static int launch_bf16(const Bf16Args& a) {
+// One instantiation per (config, B layout, output type); A_MN: A is stored transposed, [K, M] row-major;
+// Fuse: what the launch fuses to the product.
+template <class Cfg, bool B_MN, bool OUT_F32, bool A_MN = false, class Fuse = NoFuse>
+static int launch_bf16_fused(const Bf16Args& a, const Fuse& fuse) {
   constexpr int CG = Cfg::CG;
   DeviceInfo di;
   if (int rc = device_info(&di)) return rc;
@@ -402,7 +405,7 @@ static int launch_bf16(const Bf16Args& a) {
     tmC = tmA;   // unused by the kernel
   }
 
-  auto kern = gemm_bf16_kernel<Cfg, B_MN, OUT_F32, A_MN>;
+  auto kern = gemm_bf16_kernel<Cfg, B_MN, OUT_F32, A_MN, Fuse>;
   int max_clusters = 0;
   if (int rc = persistent_clusters(kern, CG, Cfg::THREADS, Cfg::SMEM_BYTES, di, &max_clusters)) return rc;
 
@@ -448,7 +451,12 @@ static int launch_bf16(const Bf16Args& a) {
     return fail(GEMM_B200_ERR_INVALID_ARG, "gemm_bf16: K splits run on the static schedule");
 
   static const GroupTable no_groups = {};   // count == 0
-  return launch_clusters(kern, clusters, CG, Cfg::THREADS, Cfg::SMEM_BYTES, a.stream, tmA, tmB, tmC, a.C, a.ldc, shape, no_groups);
+  return launch_clusters(kern, clusters, CG, Cfg::THREADS, Cfg::SMEM_BYTES, a.stream, tmA, tmB, tmC, a.C, a.ldc, shape, no_groups, fuse);
+}
+
+template <class Cfg, bool B_MN, bool OUT_F32, bool A_MN = false>
+static int launch_bf16(const Bf16Args& a) {
+  return launch_bf16_fused<Cfg, B_MN, OUT_F32, A_MN>(a, NoFuse());
 }
 
 // Grouped (ragged) BF16 GEMM, at most kMaxGroups groups per launch: single-CTA 128 x 256 tiles with
@@ -507,7 +515,7 @@ static int launch_bf16_grouped(const void* A, const void* B, void* C, int groups
   shape.c_batch_stride = 0;
   shape.l2_stream_a_keep_b = 0;
   const int clusters = (int)(tiles < max_clusters ? tiles : max_clusters);
-  return launch_clusters(kern, clusters, 1, Cfg::THREADS, Cfg::SMEM_BYTES, stream, tmA, tmB, tmA, C, ldc, shape, table);
+  return launch_clusters(kern, clusters, 1, Cfg::THREADS, Cfg::SMEM_BYTES, stream, tmA, tmB, tmA, C, ldc, shape, table, NoFuse());
 }
 
 struct Bf16ConfigEntry {
@@ -1669,6 +1677,8 @@ extern "C" int gemm_b200_gemm_mxfp8_splitk_static(const void* Aq, const void* SF
   return gemm_b200_gemm_mxfp8_splitk(Aq, SFA, Bq, SFB, C, M, N, K, ldc, out_dtype, k_splits, scratch,
                                      (size_t)GEMM_B200_STATIC_SCRATCH_BYTES, stream);
 }
+
+#include "fused_host.cuh"
 
 // =========================================================================================
 // Self-test of the bounded-wait / status path

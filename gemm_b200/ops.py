@@ -17,6 +17,7 @@ __all__ = [
     "sgemm_f32", "sgemm_f32_batched", "gemm_bf16", "gemm_bf16_batched", "gemm_bf16_grouped", "gemm_bf16_at", "check_status", "sgemm_f32_host", "gemm_bf16_host",
     "sgemm_f32_configs", "gemm_bf16_configs", "launch_count",
     "quantize_mxfp8", "gemm_mxfp8", "gemm_mxfp8_configs", "MxFp8Tensor", "gemm_mxfp8_splitk", "gemm_mxfp8_auto_splits", "gemm_mxfp8_quant_out", "gemm_mxfp8_grouped", "quantize_mxfp8_stack",
+    "gemm_bf16_xent", "gemm_bf16_xent_grad", "gemm_bf16_lora", "gemm_bf16_lora_grad",
 ]
 
 
@@ -249,6 +250,151 @@ def gemm_bf16_grouped(A: torch.Tensor, B: torch.Tensor, m_sizes, out: torch.Tens
                                               _row_major_ld(out), _lib.B_ROW_MAJOR_NK if b_is_nk else _lib.B_ROW_MAJOR_KN,
                                               _lib.OUT_F32 if out_dtype == torch.float32 else _lib.OUT_BF16, _stream(A)))
     return out
+
+
+def _vector(t: torch.Tensor, n: int, dtype: torch.dtype, device: torch.device, name: str, strided: bool = False) -> None:
+    _require(t.device == device and t.dtype == dtype and t.dim() == 1 and t.shape[0] == n and (strided or n <= 1 or t.stride(0) == 1),
+             f"{name} must be a {'' if strided else 'contiguous '}1-D {dtype} tensor of {n} elements on {device}")
+
+
+def _scratch(nbytes: int, device: torch.device) -> torch.Tensor:
+    # from torch's allocator, per call: private to the call's stream, and to the graph a capture makes
+    return torch.empty((max(int(nbytes), 1),), device=device, dtype=torch.uint8)
+
+
+def _xent_operands(X: torch.Tensor, W: torch.Tensor, labels: torch.Tensor) -> tuple[int, int, int]:
+    _require(X.is_cuda and W.device == X.device, "X and W must be CUDA tensors on one device")
+    _require(X.dtype == torch.bfloat16 and W.dtype == torch.bfloat16, "expected bfloat16")
+    _require(X.dim() == 2 and W.dim() == 2 and X.shape[1] == W.shape[1], f"X is {tuple(X.shape)} but W is {tuple(W.shape)}")
+    T, D = X.shape
+    _vector(labels, T, torch.int64, X.device, "labels")
+    return T, W.shape[0], D
+
+
+def gemm_bf16_xent(X: torch.Tensor, W: torch.Tensor, labels: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """Softmax cross entropy of the logits ``X @ W.T`` without keeping them: ``(loss, lse)``, FP32 ``[T]``.
+
+    ``X`` is ``[T, D]``, ``W`` the vocabulary projection ``[V, D]``, ``labels`` int64 ``[T]``;
+    ``lse[t] = log(sum_v exp(logit[t, v]))`` and ``loss[t] = lse[t] - logit[t, labels[t]]``.  A negative label
+    (padding) has loss 0; a label >= V makes its loss NaN.  Logits, maxima and sums are FP32."""
+    T, V, D = _xent_operands(X, W, labels)
+    loss = torch.empty((T,), device=X.device, dtype=torch.float32)
+    lse = torch.empty((T,), device=X.device, dtype=torch.float32)
+    nbytes = lib.gemm_b200_gemm_bf16_xent_scratch_bytes(T, V)
+    scratch = _scratch(nbytes, X.device)
+    with _OnDevice(X.device):
+        check(lib.gemm_b200_gemm_bf16_xent(X.data_ptr(), W.data_ptr(), labels.data_ptr(), loss.data_ptr(), lse.data_ptr(), T, V, D,
+                                           _row_major_ld(X), _row_major_ld(W), scratch.data_ptr(), nbytes, _stream(X)))
+    return loss, lse
+
+
+def gemm_bf16_xent_grad(X: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor, grad_loss: torch.Tensor,
+                        grad_lse: torch.Tensor | None = None,
+                        out: tuple[torch.Tensor, torch.Tensor] | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Gradient of ``gemm_bf16_xent``: ``(dX, dW)`` in bfloat16, from ``lse`` as that call returned it.
+
+    ``grad_loss`` (and ``grad_lse``, for a loss that uses the log-sum-exp too) are FP32 ``[T]`` of any stride, so
+    the expanded scalar that a sum's gradient is goes in as it is.  The logits are recomputed a piece of the
+    vocabulary at a time.  A row whose gradients are zero, as padding's are, adds nothing to ``dW`` whatever
+    its ``X`` holds.  ``grad_loss`` is not read where the label is negative; a label >= V makes its
+    row of ``dX``, and ``dW``, NaN."""
+    T, V, D = _xent_operands(X, W, labels)
+    _vector(lse, T, torch.float32, X.device, "lse")
+    _vector(grad_loss, T, torch.float32, X.device, "grad_loss", strided=True)
+    if grad_lse is not None:
+        _vector(grad_lse, T, torch.float32, X.device, "grad_lse", strided=True)
+    if out is None:
+        dX = torch.empty((T, D), device=X.device, dtype=torch.bfloat16)
+        dW = torch.empty((V, D), device=X.device, dtype=torch.bfloat16)
+    else:
+        dX, dW = out
+        for t, rows in ((dX, T), (dW, V)):
+            _require(t.device == X.device and t.dtype == torch.bfloat16 and tuple(t.shape) == (rows, D), "bad out tensor")
+    with _OnDevice(X.device):
+        nbytes = lib.gemm_b200_gemm_bf16_xent_grad_scratch_bytes(T, V, D)
+        scratch = _scratch(nbytes, X.device)
+        check(lib.gemm_b200_gemm_bf16_xent_grad(
+            X.data_ptr(), W.data_ptr(), labels.data_ptr(), lse.data_ptr(), grad_loss.data_ptr(), grad_loss.stride(0),
+            0 if grad_lse is None else grad_lse.data_ptr(), 0 if grad_lse is None else grad_lse.stride(0), dX.data_ptr(), dW.data_ptr(),
+            T, V, D, _row_major_ld(X), _row_major_ld(W), _row_major_ld(dX), _row_major_ld(dW), scratch.data_ptr(), nbytes, _stream(X)))
+    return dX, dW
+
+
+def _lora_operands(X, A, B, ids, scales, N: int) -> tuple[int, int, int, int, int, int, int, int]:
+    _require(X.is_cuda and A.device == X.device and B.device == X.device, "X, A and B must be CUDA tensors on one device")
+    _require(X.dtype == torch.bfloat16 and A.dtype == torch.bfloat16 and B.dtype == torch.bfloat16, "expected bfloat16")
+    _require(X.dim() == 2 and A.dim() == 3 and B.dim() == 3, "X must be 2-D, A and B 3-D")
+    T, D = X.shape
+    n, R = A.shape[0], A.shape[1]
+    _require(A.shape[2] == D and B.shape[0] == n and B.shape[1] == R and B.shape[2] == N,
+             f"X is {tuple(X.shape)}, A {tuple(A.shape)}, B {tuple(B.shape)}, and the projection has {N} columns")
+    _vector(ids, T, torch.int32, X.device, "ids")
+    if scales is not None:
+        _vector(scales, n, torch.float32, X.device, "scales")
+    lda, sa = _batch_layout(A)
+    ldb, sb = _batch_layout(B)
+    if n == 1:   # the stride of a dimension of one element means nothing
+        sa, sb = R * lda, R * ldb
+    return T, D, n, R, lda, sa, ldb, sb
+
+
+def gemm_bf16_lora(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.Tensor, ids: torch.Tensor,
+                   scales: torch.Tensor | None = None, out: torch.Tensor | None = None, *, b_is_nk: bool = False,
+                   out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """A projection shared by many requests, each with a low-rank adapter of its own:
+    ``out[t] = X[t] @ W + scales[a] * (X[t] @ A[a].T) @ B[a]`` with ``a = ids[t]``.
+
+    ``X`` is ``[T, D]``; ``W`` is ``[D, N]`` or, with ``b_is_nk``, ``[N, D]``; ``A`` is ``[n, R, D]`` and ``B`` ``[n, R, N]`` with
+    R <= 128 (pad smaller ranks with zeros); ``ids`` is int32 ``[T]`` on the device, in any order, and a negative id
+    means no adapter; ``scales`` is FP32 ``[n]``.  An id >= n makes its row NaN.  Rows of one adapter are
+    cheapest next to each other.  The gradient with respect to X is the same operator,
+    ``gemm_bf16_lora(dY, W, B, A, ids, scales, b_is_nk=not b_is_nk)``."""
+    _require(W.device == X.device and W.dtype == torch.bfloat16 and W.dim() == 2, "W must be a 2-D CUDA bfloat16 tensor")
+    _require(out_dtype in (torch.bfloat16, torch.float32), "out_dtype must be bfloat16 or float32")
+    N = W.shape[0] if b_is_nk else W.shape[1]
+    T, D, n, R, lda, sa, ldb, sb = _lora_operands(X, A, B, ids, scales, N)
+    _require(W.shape[1 if b_is_nk else 0] == D, f"X is {tuple(X.shape)} but W is {tuple(W.shape)}")
+    if out is None:
+        out = torch.empty((T, N), device=X.device, dtype=out_dtype)
+    _require(out.device == X.device and out.dtype == out_dtype and tuple(out.shape) == (T, N), "bad out tensor")
+    od = _lib.OUT_F32 if out_dtype == torch.float32 else _lib.OUT_BF16
+    with _OnDevice(X.device):
+        nbytes = lib.gemm_b200_gemm_bf16_lora_scratch_bytes(T, N, D, R, od)
+        scratch = _scratch(nbytes, X.device)
+        check(lib.gemm_b200_gemm_bf16_lora(
+            X.data_ptr(), W.data_ptr(), A.data_ptr(), B.data_ptr(), ids.data_ptr(), 0 if scales is None else scales.data_ptr(),
+            out.data_ptr(), T, N, D, R, n, _row_major_ld(X), _row_major_ld(W), lda, sa, ldb, sb, _row_major_ld(out),
+            _lib.B_ROW_MAJOR_NK if b_is_nk else _lib.B_ROW_MAJOR_KN, od, scratch.data_ptr(), nbytes, _stream(X)))
+    return out
+
+
+def gemm_bf16_lora_grad(X: torch.Tensor, dY: torch.Tensor, A: torch.Tensor, B: torch.Tensor, ids: torch.Tensor,
+                        scales: torch.Tensor | None = None, out: tuple[torch.Tensor, torch.Tensor] | None = None, *,
+                        out_dtype: torch.dtype = torch.bfloat16) -> tuple[torch.Tensor, torch.Tensor]:
+    """Gradients of the adapters of ``gemm_bf16_lora``: ``(dA, dB)``, contiguous ``[n, R, D]`` and ``[n, R, N]`` in bfloat16 or
+    FP32, for the output gradient ``dY`` ``[T, N]``.  Rows with an id outside [0, n) add nothing; adapters without a
+    row get zeros.  The order of every sum is fixed."""
+    _require(dY.device == X.device and dY.dtype == torch.bfloat16 and dY.dim() == 2 and dY.shape[0] == X.shape[0],
+             "dY must be a 2-D CUDA bfloat16 tensor with the rows of X")
+    _require(out_dtype in (torch.bfloat16, torch.float32), "out_dtype must be bfloat16 or float32")
+    N = dY.shape[1]
+    T, D, n, R, lda, sa, ldb, sb = _lora_operands(X, A, B, ids, scales, N)
+    if out is None:
+        dA = torch.empty((n, R, D), device=X.device, dtype=out_dtype)
+        dB = torch.empty((n, R, N), device=X.device, dtype=out_dtype)
+    else:
+        dA, dB = out
+        for t, like in ((dA, A), (dB, B)):
+            _require(t.device == X.device and t.dtype == out_dtype and t.shape == like.shape and t.is_contiguous(), "bad out tensor")
+    od = _lib.OUT_F32 if out_dtype == torch.float32 else _lib.OUT_BF16
+    with _OnDevice(X.device):
+        nbytes = lib.gemm_b200_gemm_bf16_lora_grad_scratch_bytes(T, N, D, R, n, od)
+        scratch = _scratch(nbytes, X.device)
+        check(lib.gemm_b200_gemm_bf16_lora_grad(
+            X.data_ptr(), dY.data_ptr(), A.data_ptr(), B.data_ptr(), ids.data_ptr(), 0 if scales is None else scales.data_ptr(),
+            dA.data_ptr(), dB.data_ptr(), T, N, D, R, n, _row_major_ld(X), _row_major_ld(dY), lda, sa, ldb, sb, od,
+            scratch.data_ptr(), nbytes, _stream(X)))
+    return dA, dB
 
 
 def check_status(device: torch.device | None = None) -> None:

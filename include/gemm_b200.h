@@ -175,6 +175,69 @@ int gemm_b200_gemm_bf16_grouped(const void* A, const void* B, void* C, int64_t g
                                 int b_layout, int out_dtype, void* stream);
 
 /* -------------------------------------------------------------------------
+ * Softmax cross entropy over a vocabulary projection, without keeping the logits:
+ *   z = X[T,D] @ W[V,D]^T,   lse_t = log sum_v exp(z_tv),   loss_t = lse_t - z_t,labels[t]
+ * X and W bf16 row-major; labels int64 on the device; loss and lse FP32 [T].  A negative label
+ * (padding) has loss 0, a label >= V has loss NaN; lse is written for every row.  Logits, maxima and
+ * sums are FP32; the order of every sum is fixed.
+ * `scratch`: device memory of gemm_b200_gemm_bf16_xent_scratch_bytes() bytes, 256-byte aligned, the
+ * caller's; its contents mean nothing before or after the call.  The reference has no loss; the
+ * product extends its operator (naive/naive.cpp:6-22).
+ * Requirements: X and W 16-byte aligned, ldx and ldw multiples of 8.
+ * ------------------------------------------------------------------------- */
+int gemm_b200_gemm_bf16_xent(const void* X, const void* W, const int64_t* labels, float* loss, float* lse,
+                             int64_t T, int64_t V, int64_t D, int64_t ldx, int64_t ldw,
+                             void* scratch, size_t scratch_bytes, void* stream);
+size_t gemm_b200_gemm_bf16_xent_scratch_bytes(int64_t T, int64_t V);
+
+/* Its gradient, with lse as the call above wrote it:
+ *   d_tv = (g_t + h_t) exp(z_tv - lse_t) - g_t [v == labels[t]],   dX = d W,   dW = d^T X   (bf16)
+ * g = grad_loss (FP32, element t at grad_loss[t * grad_loss_stride]; taken as 0 where the label is
+ * negative), h = grad_lse (likewise; NULL = 0).  A stride of 0 is a scalar.  The logits are recomputed a
+ * piece of the vocabulary at a time; d is rounded to bf16 between the products.  A row with g = h = 0
+ * adds nothing to dW whatever X holds there; a label >= V makes its row of dX, and dW, NaN.
+ * The outputs may not overlap the inputs or each other.  Requirements: as above, also for dX and dW;
+ * D a multiple of 8.  The scratch size is for the current device. */
+int gemm_b200_gemm_bf16_xent_grad(const void* X, const void* W, const int64_t* labels, const float* lse,
+                                  const float* grad_loss, int64_t grad_loss_stride,
+                                  const float* grad_lse, int64_t grad_lse_stride, void* dX, void* dW,
+                                  int64_t T, int64_t V, int64_t D, int64_t ldx, int64_t ldw, int64_t lddx, int64_t lddw,
+                                  void* scratch, size_t scratch_bytes, void* stream);
+size_t gemm_b200_gemm_bf16_xent_grad_scratch_bytes(int64_t T, int64_t V, int64_t D);
+
+/* -------------------------------------------------------------------------
+ * Low-rank adapters of many requests beside a shared projection:
+ *   Y[t] = X[t] @ W + scales[a] * (X[t] @ A_a^T) @ B_a,   a = ids[t]
+ * X bf16 [T,D]; W as B of gemm_b200_gemm_bf16 (w_layout); A_a = A + a * stride_a, [R,D] with pitch lda;
+ * B_a = B + a * stride_b, [R,N] with pitch ldb; ids int32 [T] on the device, in any order; scales FP32
+ * [adapters] on the device (NULL = 1).  A negative id means no adapter, an id >= adapters makes its row
+ * NaN.  Infinities and NaN in one adapter reach only the rows that use it.  R <= 128.
+ * X A^T is kept as one bf16 value for bf16 output and as three summands (24 bits) for FP32 output.
+ * The gradient with respect to X is the same call with dY for X, W in the other layout, and A and B
+ * exchanged.  The reference has no counterpart; the product extends its operator
+ * (naive/naive.cpp:6-22).
+ * Requirements: pointers 16-byte aligned; D, N, every leading dimension and stride multiples of 8 (ldy * sizeof(Y)
+ * of 16 bytes); scratch as above.
+ * ------------------------------------------------------------------------- */
+int gemm_b200_gemm_bf16_lora(const void* X, const void* W, const void* A, const void* B, const int32_t* ids,
+                             const float* scales, void* Y, int64_t T, int64_t N, int64_t D, int64_t R, int64_t adapters,
+                             int64_t ldx, int64_t ldw, int64_t lda, int64_t stride_a, int64_t ldb, int64_t stride_b,
+                             int64_t ldy, int w_layout, int out_dtype, void* scratch, size_t scratch_bytes, void* stream);
+size_t gemm_b200_gemm_bf16_lora_scratch_bytes(int64_t T, int64_t N, int64_t D, int64_t R, int out_dtype);
+
+/* Gradients of the adapters for the output gradient dY[T,N]:
+ *   dA_a = scales[a] * sum_{t: ids[t] = a} (dY[t] B_a^T)^T X[t],   dB_a = scales[a] * sum (X[t] A_a^T)^T dY[t]
+ * dA [adapters][R][D] and dB [adapters][R][N] contiguous, bf16 or FP32 (out_dtype).  Rows whose id is outside
+ * [0, adapters) add nothing; adapters without a row get zeros.  Sums are FP32 in a fixed order.  At most
+ * 65535 adapters; otherwise as above. */
+int gemm_b200_gemm_bf16_lora_grad(const void* X, const void* dY, const void* A, const void* B, const int32_t* ids,
+                                  const float* scales, void* dA, void* dB, int64_t T, int64_t N, int64_t D, int64_t R,
+                                  int64_t adapters, int64_t ldx, int64_t lddy, int64_t lda, int64_t stride_a,
+                                  int64_t ldb, int64_t stride_b, int out_dtype,
+                                  void* scratch, size_t scratch_bytes, void* stream);
+size_t gemm_b200_gemm_bf16_lora_grad_scratch_bytes(int64_t T, int64_t N, int64_t D, int64_t R, int64_t adapters, int out_dtype);
+
+/* -------------------------------------------------------------------------
  * MXFP8 (OCP microscaling): e4m3 data with one UE8M0 scale per 32 consecutive
  * K elements.  No counterpart in the reference; same operator semantics as
  * above (naive/naive.cpp:6-22) on quantised operands.
