@@ -90,9 +90,10 @@ static bool bf16_pairs_dynamic(int64_t M, int64_t N, int64_t K, int sms) {
 // =========================================================================================
 // Softmax cross entropy
 // =========================================================================================
-using Xent_1cta = Bf16Cfg<1, 4, 0, false>;
-using Xent_2cta = Bf16Cfg<2, 7, 0, true, 1, 0>;
-using Xent_2cta_dyn = Bf16Cfg<2, 7, 0, true, 1, 0, kBlockN, true>;
+// One row tile streams W once: 128-column tiles, so that the last round of tiles over the SMs is fuller.
+using Xent_1cta = Bf16Cfg<1, 7, 0, false, 1, 0, 128, false, 8>;
+using Xent_2cta = Bf16Cfg<2, 7, 0, true, 1, 0, kBlockN, false, 8>;
+using Xent_2cta_dyn = Bf16Cfg<2, 7, 0, true, 1, 0, kBlockN, true, 8>;
 
 struct XentScratch {
   float2* part;
@@ -100,7 +101,7 @@ struct XentScratch {
   size_t bytes;
   XentScratch(void* base, int64_t T, int64_t V) {
     Carver c{static_cast<char*>(base)};
-    part = c.take<float2>(ceil_div64(V, kBlockN) * T);
+    part = c.take<float2>(ceil_div64(V, kXentCols) * T);
     label_logit = c.take<float>(T);
     bytes = c.used;
   }
@@ -179,8 +180,12 @@ static int xent_entry(const void* X, const void* W, const int64_t* labels, float
   else if (bf16_pairs_dynamic(T, V, D, di.sms)) rc = launch_bf16_fused<Xent_2cta_dyn, false, true>(a, fuse);
   else rc = launch_bf16_fused<Xent_2cta, false, true>(a, fuse);
   if (rc) return rc;
-  return launch_plain(xent_finish_kernel, dim3((unsigned)ceil_div64(T, 32)), 32 * kXentSlices, 0, 1, st, (const float2*)ws.part,
-                      (const float*)ws.label_logit, labels, loss, lse, (int)T, (int)ceil_div64(V, kBlockN), (int)V);
+  const int groups = (int)ceil_div64(V, kXentCols);
+  auto finish = [&](auto kern, int rows) {
+    return launch_plain(kern, dim3((unsigned)ceil_div64(T, rows)), kXentFinishThreads, 0, 1, st, (const float2*)ws.part,
+                        (const float*)ws.label_logit, labels, loss, lse, (int)T, groups, (int)V);
+  };
+  return T >= 2048 ? finish(xent_finish_kernel<32>, 32) : T >= 64 ? finish(xent_finish_kernel<4>, 4) : finish(xent_finish_kernel<1>, 1);
 }
 
 static int xent_grad_entry(const void* X, const void* W, const int64_t* labels, const float* lse, const float* grad_loss,
@@ -291,9 +296,9 @@ static int launch_shrink(ShrinkArgs args, int problems, int64_t max_k, const Dev
   auto kern = lora_shrink_kernel<MT, NT8>;
   if (int rc = allow_smem(kern, S::SMEM_BYTES, di)) return rc;
   const int64_t blocks = ceil_div64(args.T, args.rows_per_block);
-  // K over the blocks of a cluster until two blocks per SM are busy, as long as every warp keeps a step of 32 k
+  // K over the blocks of a cluster until every SM has one, as long as every warp keeps a step of 32 k
   int ks = 1;
-  while (ks < 8 && blocks * problems * args.chunks * ks < 2 * (int64_t)di.sms && max_k / 32 >= 2 * ks * kShrinkWarps) ks *= 2;
+  while (ks < kShrinkMaxCluster && 5 * blocks * problems * args.chunks * ks < 4 * (int64_t)di.sms && max_k / 32 >= 2 * ks * kShrinkWarps) ks *= 2;
   return launch_plain(kern, dim3((unsigned)blocks, (unsigned)ks, (unsigned)(problems * args.chunks)), 32 * kShrinkWarps, S::SMEM_BYTES, ks,
                       st, args);
 }
@@ -303,7 +308,7 @@ static int lora_shrink(ShrinkArgs args, int problems, int64_t max_k, const Devic
   const int cols = args.rp > 64 ? 64 : args.rp;
   // few rows: a block per row, so that every adapter streams on its own; many rows: 32 or 64 rows share the
   // adapter's fragments; between them 16
-  if (args.T < 1024) {
+  if (args.T < 512) {
     args.rows_per_block = args.T <= 64 ? 1 : 16;
     return cols == 16   ? launch_shrink<1, 2>(args, problems, max_k, di, st)
            : cols == 32 ? launch_shrink<1, 4>(args, problems, max_k, di, st)
@@ -327,11 +332,14 @@ struct LoraScratch {
   }
 };
 
-template <class Cfg>
-static int launch_lora(const Bf16Args& a, const LoraFuse& fuse, int b_layout, bool f32) {
-  if (b_layout == GEMM_B200_B_ROW_MAJOR_KN)
-    return f32 ? launch_bf16_fused<Cfg, true, true>(a, fuse) : launch_bf16_fused<Cfg, true, false>(a, fuse);
-  return f32 ? launch_bf16_fused<Cfg, false, true>(a, fuse) : launch_bf16_fused<Cfg, false, false>(a, fuse);
+// the tile shapes of bf16 results, and those of FP32 ones (accumulators drained every 512 of K)
+using Lora_1cta_f32 = Bf16Cfg<1, 6, 1, false, 1, 2, 128, false, 8>;
+using Lora_2cta_f32 = Bf16Cfg<2, 6, 1, true, 1, 1, kBlockN, false, 8>;
+using Lora_2cta_f32_dyn = Bf16Cfg<2, 6, 1, true, 1, 1, kBlockN, true, 8>;
+
+template <class Cfg, bool F32>
+static int launch_lora(const Bf16Args& a, const LoraFuse& fuse, int b_layout) {
+  return b_layout == GEMM_B200_B_ROW_MAJOR_KN ? launch_bf16_fused<Cfg, true, F32>(a, fuse) : launch_bf16_fused<Cfg, false, F32>(a, fuse);
 }
 
 static int lora_entry(const void* X, const void* W, const void* A, const void* B, const int32_t* ids, const float* scales, void* Y,
@@ -383,14 +391,21 @@ static int lora_entry(const void* X, const void* W, const void* A, const void* B
     a.C = ws.slices;
     a.ldc = N;
     a.k_splits = splits;
-    const int rc = bf16_splitk_pairs(T) ? launch_lora<Bf16_2cta_tma_m>(a, fuse, w_layout, true) : launch_lora<Bf16_1cta_tma>(a, fuse, w_layout, true);
+    int rc;
+    if (f32) rc = bf16_splitk_pairs(T) ? launch_lora<Lora_2cta_f32, true>(a, fuse, w_layout) : launch_lora<Lora_1cta_f32, true>(a, fuse, w_layout);
+    else rc = bf16_splitk_pairs(T) ? launch_lora<Bf16_2cta_tma_m, true>(a, fuse, w_layout) : launch_lora<Bf16_1cta_tma, true>(a, fuse, w_layout);
     if (rc) return rc;
     const int64_t num_kb = ceil_div64(D, kBlockK);
     return launch_splitk_reduce(ws.slices, T, N, (int)ceil_div64(num_kb, ceil_div64(num_kb, splits)), Y, ldy, out_dtype, st);
   }
-  if (T <= kBlockM) return launch_lora<Bf16_1cta_tma>(a, fuse, w_layout, f32);
-  if (bf16_pairs_dynamic(T, N, D, di.sms)) return launch_lora<Bf16_2cta_tma_m_dyn>(a, fuse, w_layout, f32);
-  return launch_lora<Bf16_2cta_tma_m>(a, fuse, w_layout, f32);
+  const bool dynamic = bf16_pairs_dynamic(T, N, D, di.sms);
+  if (f32)
+    return T <= kBlockM ? launch_lora<Lora_1cta_f32, true>(a, fuse, w_layout)
+           : dynamic    ? launch_lora<Lora_2cta_f32_dyn, true>(a, fuse, w_layout)
+                        : launch_lora<Lora_2cta_f32, true>(a, fuse, w_layout);
+  return T <= kBlockM ? launch_lora<Bf16_1cta_tma, false>(a, fuse, w_layout)
+         : dynamic    ? launch_lora<Bf16_2cta_tma_m_dyn, false>(a, fuse, w_layout)
+                      : launch_lora<Bf16_2cta_tma_m, false>(a, fuse, w_layout);
 }
 
 struct LoraGradPlan {

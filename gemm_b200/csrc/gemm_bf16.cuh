@@ -115,13 +115,19 @@ struct SchedRing {
 //     the grid has one cluster per unit, the clusters that get to run first keep running and adopt
 //     the units of clusters that have not started (cluster launch control), so the units in flight
 //     are always a contiguous window of the raster however far the clusters drift apart in time.
+// ACC_KB: K blocks summed in the tensor cores at a time; 0: all of them.  The tensor cores cut low bits off a
+//     long running sum (with K = 4096 an FP32 result is off by 4e-6 of its size, always towards zero), so results that
+//     are FP32 for their precision are drained every ACC_KB blocks and added up in registers: 128 columns per epilogue
+//     warp, 5e-7 with 8 blocks (K = 512).  The drains use the two accumulator buffers in turn, as tiles do, and hide
+//     under the next blocks' products.
 template <int CG_, int STAGES_, int EPI_, bool COMMIT_MASK_, int NT_ = 1, int EPI_BUFS_ = (NT_ == 1 ? 2 : 1),
-          int BN_ = kBlockN, bool DYN_ = false>
+          int BN_ = kBlockN, bool DYN_ = false, int ACC_KB_ = 0>
 struct Bf16Cfg {
   static constexpr int CG = CG_, STAGES = STAGES_, EPI = EPI_, NT = NT_, BN = BN_;
   static constexpr bool COMMIT_MASK = COMMIT_MASK_, DYN = DYN_;
   static constexpr int ACC_STAGES = (NT == 1) ? 2 : 1;
-  static constexpr int EPI_WARPS = 4 * NT;
+  static constexpr int ACC_KB = ACC_KB_;
+  static constexpr int EPI_WARPS = ACC_KB > 0 ? 4 * (BN / 128) : 4 * NT;
   static constexpr int THREADS = 64 + 32 * EPI_WARPS;
   static constexpr int EPI_BUFS = EPI_BUFS_;                       // staging buffers per epilogue warp
   static constexpr int TILE_N = BN * NT;                       // columns of C per work unit
@@ -137,6 +143,7 @@ struct Bf16Cfg {
   static_assert(NT == 1 || NT == 2, "column tiles per unit");
   static_assert(BN == 256 || (BN == 128 && NT == 1), "tile width");
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
+  static_assert(ACC_KB == 0 || NT == 1, "drained accumulators need two buffers");
 };
 
 struct GemmShape {
@@ -203,10 +210,11 @@ enum FuseKind : int {
 struct NoFuse { static constexpr FuseKind KIND = kFuseNone; };
 struct AddFuse { static constexpr FuseKind KIND = kFuseAdd; };
 
-// Softmax cross entropy, forward.  One pair (maximum, sum of exp(z - maximum)) per row and column
-// tile, at part[column tile * M + row], and the label's logit.  A tile without a finite maximum is kept
+// Softmax cross entropy, forward.  One pair (maximum, sum of exp(z - maximum)) per row and kXentCols
+// columns, at part[column group * M + row], and the label's logit.  A group without a finite maximum is kept
 // apart so that the rows' totals come out as log(sum(exp)) says: all -inf -> (-inf, 0), an
 // infinity -> (+inf, +inf), a NaN -> (anything, NaN).
+constexpr int kXentCols = 128;
 struct XentStatsFuse {
   static constexpr FuseKind KIND = kFuseXentStats;
   float2* part;
@@ -274,6 +282,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                  const GemmShape shape, const __grid_constant__ GroupTable groups, const __grid_constant__ Fuse fuse) {
   constexpr int CG = Cfg::CG, STAGES = Cfg::STAGES, NT = Cfg::NT, ACC_STAGES = Cfg::ACC_STAGES, BN = Cfg::BN;
   static_assert(Fuse::KIND == kFuseNone || NT == 1, "the fused forms are written for one accumulator per unit");
+  static_assert(Fuse::KIND != kFuseXentStats || Cfg::ACC_KB > 0, "the loss takes its logits from the drained accumulators");
   static_assert(Fuse::KIND != kFuseXentGrad || (Cfg::EPI == 1 && !OUT_F32), "the gradient leaves as bf16 through TMA stores");
   static_assert(Fuse::KIND != kFuseAdd || (Cfg::EPI == 1 && OUT_F32), "tiles are added in FP32 through TMA");
   extern __shared__ uint8_t smem_raw[];
@@ -366,7 +375,9 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   // the stream was still running: nothing above touches global memory, everything below may, so
   // wait here for that kernel to complete.  Then let the kernel behind this one (the split-K
   // reduction, or the next GEMM) be scheduled early in turn; it waits for this grid the same way.
-  pdl_wait();
+  // kFuseLora is always launched behind lora_shrink_kernel, which lets it be scheduled only after its own
+  // wait: everything but V is complete by then, so only the producer waits, before its first load of V.
+  if constexpr (Fuse::KIND != kFuseLora) pdl_wait();
   pdl_launch_dependents();
   if (threadIdx.x == 0) trace_stamp(1);
 
@@ -442,6 +453,7 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         const int width = min(fuse.rp, 64), per_stage = 64 / width, passes = (fuse.terms * fuse.rp + 63) / 64;
         TileIds<4 * CG> tile;
         tile.load(fuse.ids, tm * CG * kBlockM, shape.M, lane);
+        if (n == 0) pdl_wait();   // the kernel that wrote V
         int slot = 0;
         bool more = !failed;
         while (more) {
@@ -515,23 +527,37 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           mma_commit_pair(map_to_cta(bar, 1));
         }
       };
-      uint32_t it = 0, acc_it = 0;
+      uint32_t it = 0, acc_it = 0, n = 0;   // acc_it: accumulators handed to the epilogue, n: units started
       int u = cluster_id;
       while (u >= 0 && u < num_tiles && !failed) {
         int t, split, kb0, kb1;
         unit_range(u, t, split, kb0, kb1);
-        const uint32_t acc = acc_it % ACC_STAGES, aph = (acc_it / ACC_STAGES) & 1u;
+        uint32_t acc = acc_it % ACC_STAGES, aph = (acc_it / ACC_STAGES) & 1u;
         if (!mbar_wait_warp(tempty_bar(acc), aph ^ 1u, kRoleMma, 100 + (int)acc)) { failed = true; break; }
         tc_fence_after_sync();
-        const uint32_t d_tmem = tmem_base + acc * NT * BN;   // NT accumulators of 256 columns
+        uint32_t d_tmem = tmem_base + acc * NT * BN;   // NT accumulators of 256 columns
+        int kb_first = kb0;                            // first K block of the accumulator
         for (int kb = kb0; kb < kb1; ++kb, ++it) {
+          if constexpr (Cfg::ACC_KB > 0) {
+            if (kb == kb_first + Cfg::ACC_KB) {        // to the epilogue with it, and on with the other buffer
+              if (issuer) commit(tfull_bar(acc));
+              __syncwarp();
+              ++acc_it;
+              kb_first = kb;
+              acc = acc_it % ACC_STAGES;
+              aph = (acc_it / ACC_STAGES) & 1u;
+              if (!mbar_wait_warp(tempty_bar(acc), aph ^ 1u, kRoleMma, 100 + (int)acc)) { failed = true; break; }
+              tc_fence_after_sync();
+              d_tmem = tmem_base + acc * NT * BN;
+            }
+          }
           const int s = it % STAGES;
           const uint32_t ph = (it / STAGES) & 1u;
           if (!mbar_wait_warp(full_bar(s), ph, kRoleMma, s)) { failed = true; break; }
           tc_fence_after_sync();
           if (it == 0 && issuer) trace_stamp(4);
           const uint32_t a_addr = sA0 + s * Cfg::A_BYTES;
-          const uint32_t first = kb != kb0 ? 1u : 0u;
+          const uint32_t first = kb != kb_first ? 1u : 0u;
           if (issuer) {
 #pragma unroll
             for (int k = 0; k < kBlockK / kUmmaK; ++k) {
@@ -601,8 +627,9 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         if (issuer) { trace_stamp(5); commit(tfull_bar(acc)); }   // accumulator complete -> epilogue warps of both CTAs
         __syncwarp();
         ++acc_it;
+        ++n;
         if constexpr (DYN) {
-          u = ring.wait_unit(acc_it, kRoleMma);
+          u = ring.wait_unit(n, kRoleMma);
           if (u == -2) failed = true;
         } else {
           u += num_clusters;
@@ -615,14 +642,42 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
     const int nt_w = (warp - 2) >> 2;   // which 256-column accumulator this warp drains (0 when NT = 1)
     const uint32_t lane_base = (uint32_t)(quad * 32) << 16;
     const uint32_t stage0 = sEpi0 + (uint32_t)(warp - 2) * (uint32_t)Cfg::EPI_BUFS * Cfg::EPI_WARP_BUF;
-    uint32_t acc_it = 0, store_it = 0;
+    uint32_t acc_it = 0, store_it = 0, n = 0;
     int u = cluster_id;
     while (u >= 0 && u < num_tiles && !failed) {
       int t, split, kb0, kb1, tm, tn, bi, row_base, row_end;
       unit_range(u, t, split, kb0, kb1);
       decode(t, bi, tm, tn, row_base, row_end);
       const int m0 = row_base + (tm * CG + (int)cta_rank) * kBlockM + quad * 32;   // first row of this warp
-      const int n0 = (tn * NT + nt_w) * BN;
+      // first column of this warp: its accumulator's, or its 128 columns of a drained one
+      const int n0 = Cfg::ACC_KB > 0 ? tn * BN + nt_w * 128 : (tn * NT + nt_w) * BN;
+      [[maybe_unused]] float total[Cfg::ACC_KB > 0 ? 128 : 1];
+      if constexpr (Cfg::ACC_KB > 0) {
+#pragma unroll
+        for (int j = 0; j < 128; ++j) total[j] = 0.f;
+        // all but the last of the unit's accumulators; the last one is added below
+        for (int kb = kb0; kb + Cfg::ACC_KB < kb1; kb += Cfg::ACC_KB, ++acc_it) {
+          const uint32_t a = acc_it % ACC_STAGES;
+          const bool full = mbar_wait(tfull_bar(a), (acc_it / ACC_STAGES) & 1u, kRoleEpilogue, 200 + (int)a);
+          if (!__all_sync(0xffffffffu, full)) { failed = true; break; }
+          tc_fence_after_sync();
+#pragma unroll
+          for (int c = 0; c < 8; ++c) {
+            uint32_t v[16];
+            tmem_ld_32x32b_x16(tmem_base + lane_base + a * BN + nt_w * 128 + c * 16, v);
+            tmem_ld_wait();
+#pragma unroll
+            for (int j = 0; j < 16; ++j) total[c * 16 + j] += __uint_as_float(v[j]);
+          }
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) {
+            if constexpr (CG == 1) mbar_arrive(tempty_bar(a));
+            else mbar_arrive_cluster(map_to_cta(tempty_bar(a), 0));
+          }
+        }
+        if (failed) break;
+      }
       const uint32_t acc = acc_it % ACC_STAGES, aph = (acc_it / ACC_STAGES) & 1u;
       // every lane waits, and the warp moves on only if every lane saw the phase complete: the
       // TMEM loads below are warp-collective and must not run with part of the warp missing
@@ -630,50 +685,68 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
       if (!__all_sync(0xffffffffu, ready)) { failed = true; break; }
       tc_fence_after_sync();
       if (warp == 2 && lane == 0) trace_stamp(6);
-      const uint32_t t_addr = tmem_base + lane_base + (acc * NT + nt_w) * BN;
+      const uint32_t t_addr = tmem_base + lane_base + (Cfg::ACC_KB > 0 ? acc * BN + nt_w * 128 : (acc * NT + nt_w) * BN);
       bool released = false;   // TMEM already handed back inside the branch below
       const int row = m0 + lane;
 
+      if constexpr (Cfg::ACC_KB > 0) {
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          uint32_t v[16];
+          tmem_ld_32x32b_x16(t_addr + c * 16, v);
+          tmem_ld_wait();
+#pragma unroll
+          for (int j = 0; j < 16; ++j) total[c * 16 + j] += __uint_as_float(v[j]);
+        }
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          if constexpr (CG == 1) mbar_arrive(tempty_bar(acc));
+          else mbar_arrive_cluster(map_to_cta(tempty_bar(acc), 0));
+        }
+        released = true;
+      }
+
       if constexpr (Fuse::KIND == kFuseXentStats) {
-        // One row per lane; the running maximum and sum of a softmax over the tile, 32 columns at a time.
+        // One row per lane; the running maximum and sum of a softmax over the warp's columns, 32 at a time.
         constexpr float kLog2e = 1.4426950408889634f;
         const int64_t label64 = row < row_end ? fuse.labels[row] : -1;
-        const int label = (label64 >= n0 && label64 < (int64_t)n0 + BN && label64 < shape.N) ? (int)label64 : -1;
+        const int label = (label64 >= n0 && label64 < (int64_t)n0 + kXentCols && label64 < shape.N) ? (int)label64 : -1;
         float top = -INFINITY, sum = 0.f, hit = 0.f;
-#pragma unroll 1
-        for (int c = 0; c < BN / 32; ++c) {
+#pragma unroll
+        for (int c = 0; c < kXentCols / 32; ++c) {
           const int col = n0 + c * 32;
           if (col >= shape.N) break;
-          uint32_t v[32];
-          tmem_ld_32x32b_x32(t_addr + c * 32, v);
-          tmem_ld_wait();
+          float v[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = total[c * 32 + j];
           if (col + 32 > shape.N) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (col + j >= shape.N) v[j] = 0xff800000u;   // -inf: no column
+              if (col + j >= shape.N) v[j] = -INFINITY;   // no column
           }
           float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], __uint_as_float(v[j]));
+          for (int j = 0; j < 32; ++j) mx[j & 3] = fmaxf(mx[j & 3], v[j]);
           const float now = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
           const float base = isinf(now) ? 0.f : now;       // exp(-inf - 0) = 0, exp(inf - 0) = inf: no NaN of our making
           const float nb = -base * kLog2e;
           sum = sum * (isinf(top) ? 1.f : exp2_approx(fmaf(top, kLog2e, nb)));   // top = -inf: the sum is 0 or NaN
           float part[4] = {sum, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int j = 0; j < 32; ++j) part[j & 3] += exp2_approx(fmaf(__uint_as_float(v[j]), kLog2e, nb));
+          for (int j = 0; j < 32; ++j) part[j & 3] += exp2_approx(fmaf(v[j], kLog2e, nb));
           sum = (part[0] + part[1]) + (part[2] + part[3]);
           top = now;
           if (label >= col && label < col + 32) {
 #pragma unroll
             for (int j = 0; j < 32; ++j)
-              if (col + j == label) hit = __uint_as_float(v[j]);
+              if (col + j == label) hit = v[j];
           }
         }
-        if (row < row_end) {
-          const long long n_part = (long long)shape.tiles_n * shape.M;
+        if (row < row_end && n0 < shape.N) {
+          const long long n_part = (long long)((shape.N + kXentCols - 1) / kXentCols) * shape.M;
           (void)n_part;
-          float2* dst = fuse.part + (int64_t)tn * shape.M + row;
+          float2* dst = fuse.part + (int64_t)(n0 / kXentCols) * shape.M + row;
           if (GEMM_B200_IN_BOUNDS(dst, fuse.part, n_part * 8, 8, 40)) *dst = make_float2(top, sum);
           if (label >= 0 && GEMM_B200_IN_BOUNDS(fuse.label_logit + row, fuse.label_logit, (long long)shape.M * 4, 4, 41))
             fuse.label_logit[row] = hit;
@@ -765,8 +838,10 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           if (row < row_end) xr = fuse.rows[row];
         }
         (void)xr;
-#pragma unroll 1
-        for (int c = 0; c < BN / SLAB_COLS; ++c, ++store_it) {
+        constexpr int SLABS = (Cfg::ACC_KB > 0 ? 128 : BN) / SLAB_COLS;
+        static_assert(Cfg::ACC_KB == 0 || OUT_F32, "accumulators are drained for FP32 results");
+#pragma unroll(Cfg::ACC_KB > 0 ? SLABS : 1)
+        for (int c = 0; c < SLABS; ++c, ++store_it) {
           const uint32_t buf = stage0 + (store_it % Cfg::EPI_BUFS) * Cfg::EPI_WARP_BUF;
           // the store that last read this buffer was committed EPI_BUFS slabs ago
           if (lane == 0) tma_store_wait_read<Cfg::EPI_BUFS - 1>();
@@ -775,8 +850,13 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           const uint32_t sw = (uint32_t)(lane & 7);
           if constexpr (OUT_F32) {
             uint32_t v[32];
-            tmem_ld_32x32b_x32(t_addr + c * 32, v);
-            tmem_ld_wait();
+            if constexpr (Cfg::ACC_KB > 0) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = __float_as_uint(total[c * 32 + j]);
+            } else {
+              tmem_ld_32x32b_x32(t_addr + c * 32, v);
+              tmem_ld_wait();
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j)
               asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row_addr + (((uint32_t)j ^ sw) << 4)),
@@ -838,8 +918,9 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         }
       }
       ++acc_it;
+      ++n;
       if constexpr (DYN) {
-        u = ring.wait_unit(acc_it, kRoleEpilogue);
+        u = ring.wait_unit(n, kRoleEpilogue);
         if (u == -2) failed = true;
       } else {
         u += num_clusters;

@@ -28,7 +28,6 @@ __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t add
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ uint4 ldg_16(const void* p) { return __ldg(reinterpret_cast<const uint4*>(p)); }
 __device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr) : "memory");
@@ -43,11 +42,12 @@ __device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) {
 //
 // One block: up to 16 * MT rows and, in a cluster of gridDim.y blocks, a share of K.  Its eight warps are
 // dealt out to the distinct adapters of the rows first and to K second, so that a block of one
-// request and a block of sixteen keep the same number of loads in flight.  A warp loads its fragments
-// straight from global memory, 16 bytes per lane: the order of k inside a product is free, so a lane's eight consecutive k
-// become the k pairs of two MMAs in the same way for X and A.  A row is loaded only under its
-// own adapter.  Every warp leaves its rows' sums in a buffer of its own; the final pass adds them over
-// the warps and the cluster in a fixed order.
+// request and a block of sixteen keep the same number of loads in flight.  The order of k inside a product is free, so
+// a lane's sixteen bytes of a row (eight consecutive k) become the k pairs of two MMAs, in the same way for X
+// and A, and no lane ever needs what another one loaded: every lane copies its own fragments into a ring in
+// shared memory (cp.async, three steps of 32 k deep) and waits only for itself.  A row is loaded
+// only under its own adapter.  Every warp leaves its rows' sums in a buffer of its own; they are added over the
+// warps and then over the cluster in a fixed order.
 // ---------------------------------------------------------------------------------------
 struct ShrinkProblem {
   const __nv_bfloat16* X;
@@ -62,22 +62,37 @@ struct ShrinkArgs {
   const float* scales;   // may be null: 1
   int T, R, n, rp, terms, rows_per_block, chunks;   // chunks of 64 ranks
 };
-constexpr int kShrinkWarps = 8;
+constexpr int kShrinkWarps = 8, kShrinkStages = 3, kShrinkMaxCluster = 8;
 
 template <int MT, int NT8>
 struct ShrinkShape {
   static constexpr int ROWS = 16 * MT, COLS = 8 * NT8, LD = COLS + 8;
-  static constexpr int SMEM_BYTES = kShrinkWarps * ROWS * LD * 4;
-  static constexpr int UNROLL = (2 * MT + NT8 <= 6) ? 4 : 2;
+  static constexpr int LOADS = 2 * MT + NT8;                                // 16-byte pieces per lane and step
+  static constexpr int RING_BYTES = kShrinkStages * LOADS * 512;            // per warp
+  static constexpr int SMEM_BYTES = kShrinkWarps * (RING_BYTES + ROWS * LD * 4);
+  static_assert(ROWS * COLS * 4 <= kShrinkWarps * RING_BYTES, "the block's sums take the place of the rings");
+  static_assert(SMEM_BYTES <= 231424, "shared memory budget");
 };
+
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool in) {
+  const int bytes = in ? 16 : 0;   // 0: sixteen zero bytes, nothing is read
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint4 ld_shared_16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 
 template <int MT, int NT8>
 __global__ void __launch_bounds__(32 * kShrinkWarps)
 lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
   using S = ShrinkShape<MT, NT8>;
-  constexpr int WORDS = (S::ROWS + 31) / 32, U = S::UNROLL;
-  extern __shared__ float shrink_buf[];   // [warp][row][LD]
-  __shared__ int slot_of[S::ROWS];
+  constexpr int WORDS = (S::ROWS + 31) / 32;
+  extern __shared__ __align__(16) uint8_t shrink_smem[];
+  float* warp_sums = reinterpret_cast<float*>(shrink_smem + kShrinkWarps * S::RING_BYTES);   // [warp][row][LD]
+  float* block_sums = reinterpret_cast<float*>(shrink_smem);                                 // [row][COLS], once the rings are done
+  __shared__ int slot_of[S::ROWS], id_of[S::ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int rank = blockIdx.y, ranks = gridDim.y;
   const int chunk = blockIdx.z % args.chunks;
@@ -89,13 +104,20 @@ lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
 
   TileIds<WORDS> ids;
   ids.load(args.ids, row0, row_end, lane);
+  if (warp == 0) {
+#pragma unroll
+    for (int w = 0; w < WORDS; ++w)
+      if (32 * w + lane < S::ROWS) id_of[32 * w + lane] = ids.id[w];
+  }
   int slots = 0;
   while (ids.next() >= 0) ++slots;
   ids.last = -1;
   const int by_slot = slots > 4 ? 8 : slots > 2 ? 4 : slots > 1 ? 2 : 1;
   const int by_k = kShrinkWarps / by_slot;
-  const int my_slot = warp % by_slot, my_k = rank * by_k + warp / by_slot, k_stride = ranks * by_k;
-  const int steps = (pr.K + 31) / 32;
+  const int my_slot = warp % by_slot;
+  const int steps = (pr.K + 31) / 32, per = (steps + ranks * by_k - 1) / (ranks * by_k);
+  const int step0 = min(steps, (rank * by_k + warp / by_slot) * per), step1 = min(steps, step0 + per);
+  const uint32_t ring = smem_u32(shrink_smem) + (uint32_t)(warp * S::RING_BYTES + lane * 16);
 
   for (int slot = 0; slot < slots; ++slot) {
     const int a = ids.next();
@@ -117,37 +139,53 @@ lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[mt][nt][e] = a < args.n ? 0.f : NAN;
     if (a < args.n) {
-      const __nv_bfloat16* xp[MT][2];
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) xp[mt][h] = pr.X + (int64_t)(row0 + mt * 16 + h * 8 + g) * pr.ldx + q * 8;
+      const __nv_bfloat16* xp = pr.X + (int64_t)(row0 + g) * pr.ldx + q * 8;
       const __nv_bfloat16* ap = pr.A + (int64_t)a * pr.stride_a + (int64_t)(chunk * 64 + g) * pr.lda + q * 8;
       const int ranks_left = args.R - chunk * 64 - g;
-      for (int s0 = my_k; s0 < steps; s0 += U * k_stride) {
-        uint4 x[U][MT][2], w[U][NT8];
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-          const int k = (s0 + u * k_stride) * 32;
+      auto load = [&](int step) {   // one commit group per step, an empty one past the end
+        if (step < step1) {
+          const int k = step * 32;
           const bool in = k + q * 8 < pr.K;
+          const uint32_t dst = ring + (uint32_t)(step % kShrinkStages * S::LOADS * 512);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) x[u][mt][h] = in && mine[mt][h] ? ldg_16(xp[mt][h] + k) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-          for (int nt = 0; nt < NT8; ++nt)
-            w[u][nt] = in && nt * 8 < ranks_left ? ldg_16(ap + (int64_t)(nt * 8) * pr.lda + k) : make_uint4(0u, 0u, 0u, 0u);
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int nt = 0; nt < NT8; ++nt) {
-              mma_m16n8k16_bf16(acc[mt][nt], x[u][mt][0].x, x[u][mt][1].x, x[u][mt][0].y, x[u][mt][1].y, w[u][nt].x, w[u][nt].y);
-              mma_m16n8k16_bf16(acc[mt][nt], x[u][mt][0].z, x[u][mt][1].z, x[u][mt][0].w, x[u][mt][1].w, w[u][nt].z, w[u][nt].w);
+            for (int h = 0; h < 2; ++h) {
+              const bool x_in = in && mine[mt][h];
+              cp_async_16(dst + (mt * 2 + h) * 512, x_in ? xp + (int64_t)(mt * 16 + h * 8) * pr.ldx + k : pr.X, x_in);
             }
+#pragma unroll
+          for (int nt = 0; nt < NT8; ++nt) {
+            const bool a_in = in && nt * 8 < ranks_left;
+            cp_async_16(dst + (2 * MT + nt) * 512, a_in ? ap + (int64_t)(nt * 8) * pr.lda + k : pr.A, a_in);
+          }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+#pragma unroll
+      for (int i = 0; i < kShrinkStages - 1; ++i) load(step0 + i);
+      for (int step = step0; step < step1; ++step) {
+        load(step + kShrinkStages - 1);   // into the slot this lane read two steps ago
+        asm volatile("cp.async.wait_group %0;" ::"n"(kShrinkStages - 1) : "memory");
+        const uint32_t src = ring + (uint32_t)(step % kShrinkStages * S::LOADS * 512);
+        uint4 w[NT8];
+#pragma unroll
+        for (int nt = 0; nt < NT8; ++nt) w[nt] = ld_shared_16(src + (2 * MT + nt) * 512);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          const uint4 x0 = ld_shared_16(src + (mt * 2) * 512), x1 = ld_shared_16(src + (mt * 2 + 1) * 512);
+#pragma unroll
+          for (int nt = 0; nt < NT8; ++nt) {
+            // 32 k at a time in the tensor cores (which cut off low bits of a long running sum), added up in FP32
+            float t[4] = {0.f, 0.f, 0.f, 0.f};
+            mma_m16n8k16_bf16(t, x0.x, x1.x, x0.y, x1.y, w[nt].x, w[nt].y);
+            mma_m16n8k16_bf16(t, x0.z, x1.z, x0.w, x1.w, w[nt].z, w[nt].w);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[mt][nt][e] += t[e];
+          }
+        }
       }
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -156,7 +194,7 @@ lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
         const int lr = mt * 16 + h * 8 + g;
         if (mine[mt][h]) {
           if (q == 0) slot_of[lr] = slot;   // the same value from every warp that writes it
-          float* dst = shrink_buf + (warp * S::ROWS + lr) * S::LD + 2 * q;
+          float* dst = warp_sums + (warp * S::ROWS + lr) * S::LD + 2 * q;
 #pragma unroll
           for (int nt = 0; nt < NT8; ++nt)
             *reinterpret_cast<float2*>(dst + nt * 8) = make_float2(acc[mt][nt][2 * h], acc[mt][nt][2 * h + 1]);
@@ -164,27 +202,37 @@ lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
       }
   }
   __syncthreads();
+  const int elems = (row_end - row0) * S::COLS;
+  for (int e = threadIdx.x; e < elems; e += 32 * kShrinkWarps) {
+    const int lr = e / S::COLS, c = e % S::COLS;
+    if (id_of[lr] < 0) continue;
+    float sum = 0.f;
+    for (int w = slot_of[lr] % by_slot; w < kShrinkWarps; w += by_slot) sum += warp_sums[(w * S::ROWS + lr) * S::LD + c];
+    block_sums[e] = sum;
+  }
+  __syncthreads();
   if (ranks > 1) {
     cluster_arrive();
     cluster_wait();
   }
   const int64_t ldv = (int64_t)args.terms * args.rp;
-  const uint32_t base = smem_u32(shrink_buf);
-  for (int e = rank * 32 * kShrinkWarps + threadIdx.x; e < (row_end - row0) * S::COLS; e += ranks * 32 * kShrinkWarps) {
+  const uint32_t base = smem_u32(block_sums);
+  const int share = (elems + ranks - 1) / ranks, e_end = min(elems, (rank + 1) * share);
+  for (int e = rank * share + threadIdx.x; e < e_end; e += 32 * kShrinkWarps) {
     const int lr = e / S::COLS, c = e % S::COLS, r = chunk * 64 + c;
-    const int a = args.ids[row0 + lr];
+    const int a = id_of[lr];
     if (a < 0) continue;
-    float sum = 0.f;
-    const int w0 = slot_of[lr] % by_slot;
-    for (int b = 0; b < ranks; ++b) {
-      if (ranks > 1) {
-        const uint32_t remote = map_to_cta(base, (uint32_t)b);
-        for (int w = w0; w < kShrinkWarps; w += by_slot) sum += ld_shared_cluster_f32(remote + 4u * (uint32_t)((w * S::ROWS + lr) * S::LD + c));
-      } else {
-        for (int w = w0; w < kShrinkWarps; w += by_slot) sum += shrink_buf[(w * S::ROWS + lr) * S::LD + c];
-      }
+    float v = 0.f;
+    if (ranks == 1) {
+      v = block_sums[e];
+    } else {
+      float part[kShrinkMaxCluster];
+#pragma unroll
+      for (int b = 0; b < kShrinkMaxCluster; ++b) part[b] = b < ranks ? ld_shared_cluster_f32(map_to_cta(base + 4u * (uint32_t)e, (uint32_t)b)) : 0.f;
+#pragma unroll
+      for (int b = 0; b < kShrinkMaxCluster; ++b) v += part[b];
     }
-    float v = r < args.R ? sum : 0.f;
+    v = r < args.R ? v : 0.f;
     if (a < args.n && r < args.R && args.scales) v *= args.scales[a];
     __nv_bfloat16* dst = pr.V + (row0 + lr) * ldv + r;
     const long long v_bytes = (long long)args.T * ldv * 2;
@@ -270,6 +318,7 @@ struct GradArgs {
   int n, R, block_tokens;
 };
 constexpr int kGradCols = 128, kGradTokens = 32, kGradStages = 4, kGradThreads = 128;
+constexpr int kGradRows = 8;   // steps whose row indices are held: more than the stages, so that no reader is overtaken
 
 template <int MT, int TERMS>
 struct GradShape {
@@ -291,16 +340,12 @@ struct GradWalk {
   }
 };
 
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool in) {
-  const int bytes = in ? 16 : 0;   // 0: sixteen zero bytes, nothing is read
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
-}
-
 template <int MT, int TERMS, bool OUT_F32>
 __global__ void __launch_bounds__(kGradThreads)
 lora_grad_kernel(const __grid_constant__ GradArgs args) {
   using S = GradShape<MT, TERMS>;
   extern __shared__ __align__(16) uint8_t grad_smem[];
+  __shared__ int row_ring[kGradRows][kGradTokens];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const GradProblem& pr = args.p[(int)blockIdx.x >= args.p[1].first_chunk ? 1 : 0];
   const int c0 = ((int)blockIdx.x - pr.first_chunk) * kGradCols;
@@ -315,37 +360,48 @@ lora_grad_kernel(const __grid_constant__ GradArgs args) {
     const int mid = (a0 + a1 + 1) >> 1;
     if (args.start[mid] <= lo) a0 = mid; else a1 = mid - 1;
   }
-  GradWalk ld{a0, lo, min(hi, args.start[a0 + 1]), hi};
-  ld.settle(args.start, args.n);
-  GradWalk cu = ld;
+  GradWalk ix{a0, lo, min(hi, args.start[a0 + 1]), hi};   // three walkers: row indices, loads, arithmetic
+  ix.settle(args.start, args.n);
+  GradWalk cu = ix;
 
   const uint32_t smem = smem_u32(grad_smem);
   const int64_t ldp = (int64_t)S::RP * TERMS;
-  auto load_step = [&](int stage) {   // the next step of `ld` into a stage; an empty group once it is through
-    if (ld.a < args.n) {
-      const int cnt = min(kGradTokens, ld.end - ld.pos);
-      const uint32_t qs = smem + stage * S::STAGE_BYTES, ps = qs + kGradTokens * S::Q_PITCH;
+  // the rows of the next step of `ix` (lane by lane; -1: none), one step before the loads need them
+  auto fetch_rows = [&]() -> int {
+    if (ix.a >= args.n) return -1;
+    const int cnt = min(kGradTokens, ix.end - ix.pos);
+    const int row = lane < cnt ? args.perm[ix.pos + lane] : -1;
+    ix.pos += cnt;
+    ix.settle(args.start, args.n);
+    return row;
+  };
+  auto load_step = [&](int step) {
+    const int* rows = row_ring[step % kGradRows];
+    const uint32_t qs = smem + (step % kGradStages) * S::STAGE_BYTES, ps = qs + kGradTokens * S::Q_PITCH;
+    if (rows[0] >= 0) {   // past the last step: an empty group
 #pragma unroll
       for (int i = 0; i < kGradTokens * (kGradCols / 8) / kGradThreads; ++i) {
         const int e = threadIdx.x + i * kGradThreads, t = e / (kGradCols / 8), c = e % (kGradCols / 8) * 8;
-        const bool in = t < cnt && c0 + c < pr.cols;
-        const __nv_bfloat16* src = pr.Q;
-        if (in) src += (int64_t)args.perm[ld.pos + t] * pr.ldq + c0 + c;
-        cp_async_16(qs + t * S::Q_PITCH + c * 2, src, in);
+        const int row = rows[t];
+        const bool in = row >= 0 && c0 + c < pr.cols;
+        cp_async_16(qs + t * S::Q_PITCH + c * 2, in ? pr.Q + row * pr.ldq + c0 + c : pr.Q, in);
       }
       constexpr int PV = S::RP * TERMS / 8;
-      for (int e = threadIdx.x; e < kGradTokens * PV; e += kGradThreads) {
-        const int t = e / PV, c = e % PV * 8;
-        const bool in = t < cnt;
-        const __nv_bfloat16* src = pr.P;
-        if (in) src += (int64_t)args.perm[ld.pos + t] * ldp + c;
-        cp_async_16(ps + t * S::P_PITCH + c * 2, src, in);
+#pragma unroll
+      for (int i = 0; i < (kGradTokens * PV + kGradThreads - 1) / kGradThreads; ++i) {
+        const int e = threadIdx.x + i * kGradThreads, t = e / PV, c = e % PV * 8;
+        if (kGradTokens * PV % kGradThreads == 0 || e < kGradTokens * PV) {
+          const int row = rows[t];
+          cp_async_16(ps + t * S::P_PITCH + c * 2, row >= 0 ? pr.P + row * ldp + c : pr.P, row >= 0);
+        }
       }
-      ld.pos += cnt;
-      ld.settle(args.start, args.n);
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+  if (warp == 0) {
+    for (int s = 0; s < kGradStages; ++s) row_ring[s][lane] = fetch_rows();
+  }
+  __syncthreads();
 #pragma unroll
   for (int s = 0; s < kGradStages - 1; ++s) load_step(s);
 
@@ -361,27 +417,38 @@ lora_grad_kernel(const __grid_constant__ GradArgs args) {
   clear();
   const int warp_c = warp * 32;
   for (int it = 0; cu.a < args.n; ++it) {
+    int next_row = -1;
+    if (warp == 0) next_row = fetch_rows();            // step it + kGradStages; used from the next barrier on
     asm volatile("cp.async.wait_group %0;" ::"n"(kGradStages - 2) : "memory");
     __syncthreads();
-    load_step((it + kGradStages - 1) % kGradStages);   // into the stage every warp finished with before the barrier
+    load_step(it + kGradStages - 1);                   // into the stage every warp finished with before the barrier
     const uint32_t qs = smem + (it % kGradStages) * S::STAGE_BYTES, ps = qs + kGradTokens * S::Q_PITCH;
+    uint32_t b[kGradTokens / 16][2][4];                // 32 tokens x 32 columns
 #pragma unroll
-    for (int k = 0; k < kGradTokens / 16; ++k) {
-      uint32_t b[2][4];   // 16 tokens x 32 columns
+    for (int k = 0; k < kGradTokens / 16; ++k)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        ldmatrix_x4_trans(b[h], qs + (k * 16 + (lane & 15)) * S::Q_PITCH + (warp_c + h * 16 + (lane >> 4) * 8) * 2);
+        ldmatrix_x4_trans(b[k][h], qs + (k * 16 + (lane & 15)) * S::Q_PITCH + (warp_c + h * 16 + (lane >> 4) * 8) * 2);
 #pragma unroll
-      for (int t = 0; t < TERMS; ++t)
+    for (int mt = 0; mt < MT; ++mt) {
+      // a step's products in the tensor cores (which cut off low bits of a long running sum), added up in FP32
+      float tmp[4][4] = {};
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+      for (int t = TERMS - 1; t >= 0; --t)
+#pragma unroll
+        for (int k = 0; k < kGradTokens / 16; ++k) {
           uint32_t r[4];    // P^T: 16 ranks x 16 tokens; matrices (tokens 0-7, 8-15) x (ranks 0-7, 8-15)
           ldmatrix_x4_trans(r, ps + (k * 16 + (lane >> 4) * 8 + (lane & 7)) * S::P_PITCH + (t * S::RP + mt * 16 + ((lane >> 3) & 1) * 8) * 2);
 #pragma unroll
           for (int nt = 0; nt < 4; ++nt)
-            mma_m16n8k16_bf16(acc[mt][nt], r[0], r[1], r[2], r[3], b[nt >> 1][(nt & 1) * 2], b[nt >> 1][(nt & 1) * 2 + 1]);
+            mma_m16n8k16_bf16(tmp[nt], r[0], r[1], r[2], r[3], b[k][nt >> 1][(nt & 1) * 2], b[k][nt >> 1][(nt & 1) * 2 + 1]);
         }
+#pragma unroll
+      for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[mt][nt][e] += tmp[nt][e];
     }
+    if (warp == 0) row_ring[(it + kGradStages) % kGradRows][lane] = next_row;
     cu.pos += min(kGradTokens, cu.end - cu.pos);
     if (cu.pos >= cu.end) {   // the adapter's share of this block is complete
       const int a = cu.a;

@@ -3,9 +3,8 @@
 //   z = X W^T [T, V],  lse_t = log sum_v exp(z_tv),  loss_t = lse_t - z_t,label(t)
 //   d_tv = (g_t + h_t) exp(z_tv - lse_t) - g_t [v = label(t)],  dX = d W,  dW = d^T X
 //
-// with g, h the gradients of loss and lse.  z is never kept: the forward pass reduces every 128 x 256 tile
-// of it in the epilogue of the product (XentStatsFuse in gemm_bf16.cuh) to one (maximum, sum) pair per
-// row, and the gradient recomputes it a piece of the vocabulary at a time, turning the accumulators
+// with g, h the gradients of loss and lse.  z is never kept: the forward pass reduces it in the epilogue of the
+// product (XentStatsFuse in gemm_bf16.cuh) to one (maximum, sum) pair per row and 128 columns, and the gradient recomputes it a piece of the vocabulary at a time, turning the accumulators
 // into d in the epilogue (XentGradFuse).  d is rounded to bf16 once, because the two products behind it
 // take bf16 operands; it is a relative rounding of each value (2^-9), of the size of the rounding of the
 // results themselves.
@@ -19,43 +18,72 @@
 namespace gemm_b200 {
 namespace tc {
 
-constexpr int kXentSlices = 16;   // threads that share one row's column tiles in the finishing pass
-
 // (m, s) with s a sum of exponentials relative to m; an infinite m counts as reference 0 (XentStatsFuse)
+__device__ __forceinline__ float xent_weight(float m, float base) { return isinf(m) ? 1.f : expf(m - base); }
 __device__ __forceinline__ void xent_merge(float& m, float& s, float pm, float ps) {
   const float now = fmaxf(m, pm);
   const float base = isinf(now) ? 0.f : now;
-  s = s * (isinf(m) ? 1.f : expf(m - base)) + ps * (isinf(pm) ? 1.f : expf(pm - base));
+  s = s * xent_weight(m, base) + ps * xent_weight(pm, base);
   m = now;
 }
 
-// Joins the column tiles of every row.  A block owns 32 rows (one per lane, so that the pairs of a column tile are
-// read 256 bytes at a time) and cuts the tiles into 16 interleaved slices; always the same order.
-// Bound by the read of 8 T ceil(V / 256) bytes, 1/64 of what one bf16 copy of the logits would be.
-__global__ void __launch_bounds__(32 * kXentSlices)
+// Joins the column groups of every row, always in the same order.  A block of 1024 threads owns ROWS rows: thread
+// (slice, row) takes every 1024 / ROWS-th group, eight loads at a time.  With many rows 32 of them read 256 bytes of a group
+// together; with few, the threads go along the vocabulary instead (one row of 131072 columns as one slice
+// of 16 took 14 us, as 1024 slices REPLACE_FINISH).  Bound by the read of 8 T ceil(V / 128) bytes, 1/32 of
+// a bf16 copy of the logits.
+constexpr int kXentFinishThreads = 1024;
+template <int ROWS>
+__global__ void __launch_bounds__(kXentFinishThreads)
 xent_finish_kernel(const float2* __restrict__ part, const float* __restrict__ label_logit, const int64_t* __restrict__ labels,
-                   float* __restrict__ loss, float* __restrict__ lse, int T, int tiles_n, int V) {
-  __shared__ float2 sh[kXentSlices][32];
-  const int lane = threadIdx.x & 31, slice = threadIdx.x >> 5;
-  const int row = blockIdx.x * 32 + lane;
+                   float* __restrict__ loss, float* __restrict__ lse, int T, int groups, int V) {
+  constexpr int SLICES = kXentFinishThreads / ROWS, WARPS = kXentFinishThreads / 32;
+  __shared__ float2 sh[ROWS][WARPS + 1];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int in_block = threadIdx.x % ROWS, slice = threadIdx.x / ROWS;
+  const int row = blockIdx.x * ROWS + in_block;
   pdl_wait();
   pdl_launch_dependents();
   float m = -INFINITY, s = 0.f;
   if (row < T) {
-#pragma unroll 4
-    for (int t = slice; t < tiles_n; t += kXentSlices) {
-      const float2 p = part[(int64_t)t * T + row];
-      xent_merge(m, s, p.x, p.y);
+    for (int t0 = slice; t0 < groups; t0 += 8 * SLICES) {
+      float2 p[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int t = t0 + j * SLICES;
+        p[j] = t < groups ? part[(int64_t)t * T + row] : make_float2(-INFINITY, 0.f);
+      }
+      float now = m;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) now = fmaxf(now, p[j].x);
+      const float base = isinf(now) ? 0.f : now;
+      s *= xent_weight(m, base);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += p[j].y * xent_weight(p[j].x, base);
+      m = now;
     }
   }
-  sh[slice][lane] = make_float2(m, s);
+#pragma unroll
+  for (int o = ROWS; o < 32; o *= 2) {
+    const float pm = __shfl_xor_sync(0xffffffffu, m, o), ps = __shfl_xor_sync(0xffffffffu, s, o);
+    xent_merge(m, s, pm, ps);
+  }
+  if (lane < ROWS) sh[in_block][warp] = make_float2(m, s);
   __syncthreads();
-  if (slice != 0 || row >= T) return;
-  for (int i = 1; i < kXentSlices; ++i) xent_merge(m, s, sh[i][lane].x, sh[i][lane].y);
+  if (warp >= ROWS) return;
+  m = sh[warp][lane].x;                 // warp w: row w of the block
+  s = sh[warp][lane].y;
+#pragma unroll
+  for (int o = 16; o > 0; o /= 2) {
+    const float pm = __shfl_xor_sync(0xffffffffu, m, o), ps = __shfl_xor_sync(0xffffffffu, s, o);
+    xent_merge(m, s, pm, ps);
+  }
+  const int out = blockIdx.x * ROWS + warp;
+  if (lane != 0 || out >= T) return;
   const float total = (isinf(m) ? 0.f : m) + logf(s);
-  const int64_t label = labels[row];
-  lse[row] = total;
-  loss[row] = label < 0 ? 0.f : (label >= V ? NAN : total - label_logit[row]);
+  const int64_t label = labels[out];
+  lse[out] = total;
+  loss[out] = label < 0 ? 0.f : (label >= V ? NAN : total - label_logit[out]);
 }
 
 // One block per row: the numbers the gradient epilogue needs, and the row of X for the product d^T X with
