@@ -98,9 +98,13 @@ using Xent_2cta_dyn = Bf16Cfg<2, 7, 0, true, 1, 0, kBlockN, true, 8>;
 struct XentScratch {
   float2* part;
   float* label_logit;
+  __nv_bfloat16* xp;   // X padded to kMinMapRows rows
+  int64_t ldp;
   size_t bytes;
-  XentScratch(void* base, int64_t T, int64_t V) {
+  XentScratch(void* base, int64_t T, int64_t V, int64_t D) {
     Carver c{static_cast<char*>(base)};
+    ldp = ceil_div64(D, 8) * 8;
+    xp = c.take<__nv_bfloat16>(T < kMinMapRows ? kMinMapRows * ldp : 0);
     part = c.take<float2>(ceil_div64(V, kXentCols) * T);
     label_logit = c.take<float>(T);
     bytes = c.used;
@@ -142,9 +146,10 @@ struct XentGradScratch {
   XentGradScratch(void* base, int64_t T, int64_t D, const XentGradPlan& p) {
     Carver c{static_cast<char*>(base)};
     ldd = ceil_div64(p.piece, 8) * 8;
+    const int64_t map_rows = T < kMinMapRows ? kMinMapRows : T;
     rows = c.take<XentRow>(T);
-    xw = c.take<__nv_bfloat16>(T * D);
-    d = c.take<__nv_bfloat16>(T * ldd);
+    xw = c.take<__nv_bfloat16>(map_rows * D);
+    d = c.take<__nv_bfloat16>(map_rows * ldd);
     dx = c.take<float>(p.dx_acc ? (int64_t)p.dx_splits * T * D : 0);
     dw = c.take<float>(p.dw_splits > 1 ? (int64_t)p.dw_splits * p.piece * D : 0);
     bytes = c.used;
@@ -168,14 +173,22 @@ static int xent_entry(const void* X, const void* W, const int64_t* labels, float
   if (!aligned16(X) || !aligned16(W) || ldx % 8 != 0 || ldw % 8 != 0)
     return fail(GEMM_B200_ERR_ALIGNMENT, "gemm_bf16_xent: X and W must be 16-byte aligned, ldx and ldw multiples of 8 (ldx=%lld ldw=%lld)",
                 (long long)ldx, (long long)ldw);
-  const XentScratch ws(scratch, T, V);
+  const XentScratch ws(scratch, T, V, D);
   if (int rc = check_scratch("gemm_bf16_xent", scratch, scratch_bytes, ws.bytes)) return rc;
   DeviceInfo di;
   if (int rc = check_blackwell("gemm_bf16_xent", &di)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const Bf16Args a{X, W, nullptr, T, V, D, ldx, ldw, V, st};
+  Bf16Args a{X, W, nullptr, T, V, D, ldx, ldw, V, st};
   const XentStatsFuse fuse{ws.part, ws.label_logit, labels};
   int rc;
+  if (T < kMinMapRows) {
+    if ((rc = launch_plain(xent_pad_kernel, dim3((unsigned)kMinMapRows), 128, 0, 1, st, static_cast<const __nv_bfloat16*>(X), ldx, ws.xp, ws.ldp,
+                           (int)T, (int)D)))
+      return rc;
+    a.A = ws.xp;
+    a.lda = ws.ldp;
+    a.a_rows = kMinMapRows;
+  }
   if (T <= kBlockM) rc = launch_bf16_fused<Xent_1cta, false, true>(a, fuse);
   else if (bf16_pairs_dynamic(T, V, D, di.sms)) rc = launch_bf16_fused<Xent_2cta_dyn, false, true>(a, fuse);
   else rc = launch_bf16_fused<Xent_2cta, false, true>(a, fuse);
@@ -218,15 +231,21 @@ static int xent_grad_entry(const void* X, const void* W, const int64_t* labels, 
   if (log_enabled())
     fprintf(stderr, "[gemm_b200] gemm_bf16_xent_grad T=%lld V=%lld D=%lld -> %lld pieces of %lld, K ranges %d (dX) %d (dW)\n", (long long)T,
             (long long)V, (long long)D, (long long)plan.pieces, (long long)plan.piece, plan.dx_splits, plan.dw_splits);
-  if (int rc = launch_plain(xent_prepare_kernel, dim3((unsigned)T), 128, 0, 1, st, labels, lse, grad_loss, grad_loss_stride, grad_lse,
-                            grad_lse_stride, static_cast<const __nv_bfloat16*>(X), ldx, ws.rows, ws.xw, (int)D, (int)V))
+  const int64_t a_rows = T < kMinMapRows ? kMinMapRows : 0;
+  if (int rc = launch_plain(xent_prepare_kernel, dim3((unsigned)(a_rows ? a_rows : T)), 128, 0, 1, st, labels, lse, grad_loss, grad_loss_stride,
+                            grad_lse, grad_lse_stride, static_cast<const __nv_bfloat16*>(X), ldx, ws.rows, ws.xw, (int)T, (int)D, (int)V))
     return rc;
   int dx_slices = 1;
   for (int64_t v0 = 0; v0 < V; v0 += plan.piece) {
     const int64_t n = V - v0 < plan.piece ? V - v0 : plan.piece;
     const char* Wp = static_cast<const char*>(W) + v0 * ldw * 2;
     // d of the piece
-    const Bf16Args z{X, Wp, ws.d, T, n, D, ldx, ldw, ws.ldd, st};
+    Bf16Args z{X, Wp, ws.d, T, n, D, ldx, ldw, ws.ldd, st};
+    if (a_rows) {   // rows without weight are zeros there: their logits count for nothing
+      z.A = ws.xw;
+      z.lda = D;
+      z.a_rows = a_rows;
+    }
     const XentGradFuse fuse{ws.rows, (int)v0};
     int rc;
     if (T <= kBlockM) rc = launch_bf16_fused<Bf16_1cta_tma, false, false>(z, fuse);
@@ -235,6 +254,7 @@ static int xent_grad_entry(const void* X, const void* W, const int64_t* labels, 
     if (rc) return rc;
     // dX (+)= d W
     Bf16Args gx{ws.d, Wp, dX, T, D, n, ws.ldd, ldw, lddx, st};
+    gx.a_rows = a_rows;   // rows of d above T hold anything and reach only rows of the product above T
     if (!plan.dx_acc) {
       rc = kBf16Configs[pick_bf16_config(T, D, n, di.sms)].launch[GEMM_B200_B_ROW_MAJOR_KN][GEMM_B200_OUT_BF16](gx);
     } else {
@@ -255,7 +275,10 @@ static int xent_grad_entry(const void* X, const void* W, const int64_t* labels, 
     if (plan.dw_splits > 1) {
       rc = launch_bf16_splitk(gw, GEMM_B200_B_ROW_MAJOR_KN, GEMM_B200_OUT_BF16, plan.dw_splits, ws.dw, /*a_mn=*/true);
     } else {
-      const int config = pick_bf16_config(n, D, T, di.sms);
+      // A K of a few blocks: the store of dW bounds the product, and single CTAs (two per pair to drain
+      // accumulators) store faster (dW [32001, 2048] of 67 tokens 36 us against 45, [131072, 4096] of 16 190
+      // against 286); from 512 tokens on pairs are as fast ([50001, 1024] of 509 tokens 51 / 49).
+      const int config = T <= 256 ? (int)kBf16Cfg1cta : pick_bf16_config(n, D, T, di.sms);
       rc = GEMM_B200_ERR_UNSUPPORTED;
       for (const Bf16AtEntry& e : kBf16AtConfigs)
         if (e.config == config) rc = e.launch[GEMM_B200_B_ROW_MAJOR_KN][GEMM_B200_OUT_BF16](gw);
@@ -296,9 +319,9 @@ static int launch_shrink(ShrinkArgs args, int problems, int64_t max_k, const Dev
   auto kern = lora_shrink_kernel<MT, NT8>;
   if (int rc = allow_smem(kern, S::SMEM_BYTES, di)) return rc;
   const int64_t blocks = ceil_div64(args.T, args.rows_per_block);
-  // K over the blocks of a cluster until every SM has one, as long as every warp keeps a step of 32 k
+  // K over the blocks of a cluster until most SMs have one, as long as every warp keeps a step of 64 k
   int ks = 1;
-  while (ks < kShrinkMaxCluster && 5 * blocks * problems * args.chunks * ks < 4 * (int64_t)di.sms && max_k / 32 >= 2 * ks * kShrinkWarps) ks *= 2;
+  while (ks < kShrinkMaxCluster && 5 * blocks * problems * args.chunks * ks < 4 * (int64_t)di.sms && max_k / kShrinkK >= 2 * ks * kShrinkWarps) ks *= 2;
   return launch_plain(kern, dim3((unsigned)blocks, (unsigned)ks, (unsigned)(problems * args.chunks)), 32 * kShrinkWarps, S::SMEM_BYTES, ks,
                       st, args);
 }
@@ -514,9 +537,9 @@ static int current_sms() {
 }  // namespace tc
 }  // namespace gemm_b200
 
-extern "C" size_t gemm_b200_gemm_bf16_xent_scratch_bytes(int64_t T, int64_t V) {
-  if (T <= 0 || V <= 0) return 0;
-  return gemm_b200::tc::XentScratch(nullptr, T, V).bytes;
+extern "C" size_t gemm_b200_gemm_bf16_xent_scratch_bytes(int64_t T, int64_t V, int64_t D) {
+  if (T <= 0 || V <= 0 || D <= 0) return 0;
+  return gemm_b200::tc::XentScratch(nullptr, T, V, D).bytes;
 }
 extern "C" int gemm_b200_gemm_bf16_xent(const void* X, const void* W, const int64_t* labels, float* loss, float* lse, int64_t T, int64_t V,
                                         int64_t D, int64_t ldx, int64_t ldw, void* scratch, size_t scratch_bytes, void* stream) {

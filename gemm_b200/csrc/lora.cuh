@@ -24,6 +24,14 @@ __device__ __forceinline__ void mma_m16n8k16_bf16(float (&c)[4], uint32_t a0, ui
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// the same with an accumulator of zero
+__device__ __forceinline__ void mma_m16n8k16_bf16_zero(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                                       uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};"
+      : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
 __device__ __forceinline__ void ldmatrix_x4_trans(uint32_t (&r)[4], uint32_t addr) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
@@ -42,12 +50,13 @@ __device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) {
 //
 // One block: up to 16 * MT rows and, in a cluster of gridDim.y blocks, a share of K.  Its eight warps are
 // dealt out to the distinct adapters of the rows first and to K second, so that a block of one
-// request and a block of sixteen keep the same number of loads in flight.  The order of k inside a product is free, so
-// a lane's sixteen bytes of a row (eight consecutive k) become the k pairs of two MMAs, in the same way for X
-// and A, and no lane ever needs what another one loaded: every lane copies its own fragments into a ring in
-// shared memory (cp.async, three steps of 32 k deep) and waits only for itself.  A row is loaded
-// only under its own adapter.  Every warp leaves its rows' sums in a buffer of its own; they are added over the
-// warps and then over the cluster in a fixed order.
+// request and a block of sixteen keep the same number of loads in flight.  A warp copies 64 k at a time (whole
+// 128-byte lines of eight lanes; 64-byte pieces of four lanes ran into the SM's rate of requests: 56 us
+// instead of REPLACE_SHRINK for 8192 x 8192) into two stages of its own in shared memory with cp.async and waits for
+// nobody else.  The order of k inside a product is free, so a lane reads sixteen bytes of a row (eight
+// consecutive k) as the k pairs of two MMAs, in the same way for X and A.  A row is loaded only under its
+// own adapter.  With up to eight adapters a warp has one at most and leaves its rows' sums in its own stages, to be
+// added over the warps; with more, a row belongs to one warp alone.  Then the cluster adds up.  The order is fixed.
 // ---------------------------------------------------------------------------------------
 struct ShrinkProblem {
   const __nv_bfloat16* X;
@@ -62,15 +71,15 @@ struct ShrinkArgs {
   const float* scales;   // may be null: 1
   int T, R, n, rp, terms, rows_per_block, chunks;   // chunks of 64 ranks
 };
-constexpr int kShrinkWarps = 8, kShrinkStages = 3, kShrinkMaxCluster = 8;
+constexpr int kShrinkWarps = 8, kShrinkStages = 2, kShrinkK = 64, kShrinkMaxCluster = 8;
 
 template <int MT, int NT8>
 struct ShrinkShape {
   static constexpr int ROWS = 16 * MT, COLS = 8 * NT8, LD = COLS + 8;
-  static constexpr int LOADS = 2 * MT + NT8;                                // 16-byte pieces per lane and step
-  static constexpr int RING_BYTES = kShrinkStages * LOADS * 512;            // per warp
-  static constexpr int SMEM_BYTES = kShrinkWarps * (RING_BYTES + ROWS * LD * 4);
-  static_assert(ROWS * COLS * 4 <= kShrinkWarps * RING_BYTES, "the block's sums take the place of the rings");
+  static constexpr int STAGE_ROWS = ROWS + COLS;                            // rows of 64 k: X, then A
+  static constexpr int RING_BYTES = kShrinkStages * STAGE_ROWS * 128;       // per warp
+  static constexpr int SMEM_BYTES = kShrinkWarps * RING_BYTES + ROWS * COLS * 4;
+  static_assert(ROWS * LD * 4 <= RING_BYTES, "a warp's sums take the place of its stages");
   static_assert(SMEM_BYTES <= 231424, "shared memory budget");
 };
 
@@ -84,14 +93,15 @@ __device__ __forceinline__ uint4 ld_shared_16(uint32_t addr) {
   return v;
 }
 
+__device__ __forceinline__ int shrink_swizzle(int row) { return (row & 1) << 2 | (row >> 1 & 3); }
+
 template <int MT, int NT8>
 __global__ void __launch_bounds__(32 * kShrinkWarps)
 lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
   using S = ShrinkShape<MT, NT8>;
   constexpr int WORDS = (S::ROWS + 31) / 32;
   extern __shared__ __align__(16) uint8_t shrink_smem[];
-  float* warp_sums = reinterpret_cast<float*>(shrink_smem + kShrinkWarps * S::RING_BYTES);   // [warp][row][LD]
-  float* block_sums = reinterpret_cast<float*>(shrink_smem);                                 // [row][COLS], once the rings are done
+  float* block_sums = reinterpret_cast<float*>(shrink_smem + kShrinkWarps * S::RING_BYTES);   // [row][COLS]
   __shared__ int slot_of[S::ROWS], id_of[S::ROWS];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int rank = blockIdx.y, ranks = gridDim.y;
@@ -115,22 +125,16 @@ lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
   const int by_slot = slots > 4 ? 8 : slots > 2 ? 4 : slots > 1 ? 2 : 1;
   const int by_k = kShrinkWarps / by_slot;
   const int my_slot = warp % by_slot;
-  const int steps = (pr.K + 31) / 32, per = (steps + ranks * by_k - 1) / (ranks * by_k);
-  const int step0 = min(steps, (rank * by_k + warp / by_slot) * per), step1 = min(steps, step0 + per);
-  const uint32_t ring = smem_u32(shrink_smem) + (uint32_t)(warp * S::RING_BYTES + lane * 16);
+  // K: a run of steps per block, which its warps take in turn (together they read a row 1 KB at a time)
+  const int steps = (pr.K + kShrinkK - 1) / kShrinkK, per = (steps + ranks - 1) / ranks;
+  const int step0 = min(steps, rank * per) + warp / by_slot, step1 = min(steps, (rank + 1) * per);
+  float* warp_sums = reinterpret_cast<float*>(shrink_smem + warp * S::RING_BYTES);            // [row][LD], once the stages are done
+  const uint32_t ring = smem_u32(warp_sums);
+  const int cr = lane >> 3, cc = lane & 7;   // copies: lane = (row of four, sixteen bytes of eight)
 
   for (int slot = 0; slot < slots; ++slot) {
     const int a = ids.next();
     if (slot % by_slot != my_slot) continue;
-    // which of this lane's rows have the adapter
-    bool mine[MT][2];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int lr = mt * 16 + h * 8 + g;
-        mine[mt][h] = __shfl_sync(0xffffffffu, ids.id[(mt * 16 + h * 8) / 32], lr % 32) == a;
-      }
     float acc[MT][NT8][4];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
@@ -139,62 +143,88 @@ lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
 #pragma unroll
         for (int e = 0; e < 4; ++e) acc[mt][nt][e] = a < args.n ? 0.f : NAN;
     if (a < args.n) {
-      const __nv_bfloat16* xp = pr.X + (int64_t)(row0 + g) * pr.ldx + q * 8;
-      const __nv_bfloat16* ap = pr.A + (int64_t)a * pr.stride_a + (int64_t)(chunk * 64 + g) * pr.lda + q * 8;
-      const int ranks_left = args.R - chunk * 64 - g;
-      auto load = [&](int step) {   // one commit group per step, an empty one past the end
+      uint32_t wanted = 0;   // which of the rows cr, 4 + cr, ... this lane copies
+#pragma unroll
+      for (int i = 0; i < S::ROWS / 4; ++i)
+        wanted |= (__shfl_sync(0xffffffffu, ids.id[i / 8], (i * 4 + cr) % 32) == a ? 1u : 0u) << i;
+      const __nv_bfloat16* xp = pr.X + (int64_t)(row0 + cr) * pr.ldx + cc * 8;
+      const __nv_bfloat16* ap = pr.A + (int64_t)a * pr.stride_a + (int64_t)(chunk * 64 + cr) * pr.lda + cc * 8;
+      const int ranks_left = args.R - chunk * 64 - cr;
+      const int64_t x4 = 4 * pr.ldx, a4 = 4 * pr.lda;
+      uint32_t dst_of[2];     // where this lane's copies of even and odd groups of four rows go in stage 0
+#pragma unroll
+      for (int i = 0; i < 2; ++i) dst_of[i] = ring + (uint32_t)(cr * 128 + ((cc ^ shrink_swizzle(i * 4 + cr)) << 4));
+      // 128-byte rows; sixteen-byte unit u of row r sits at unit u ^ shrink_swizzle(r): a read takes four units of
+      // eight rows, and any two neighbouring rows then lie in different halves of the banks.  Rows of another adapter
+      // and ranks above R are not copied: what the stage holds there reaches only sums that nobody reads.
+      auto load = [&](int step, int stage) {   // one commit group per step, an empty one past the end
         if (step < step1) {
-          const int k = step * 32;
-          const bool in = k + q * 8 < pr.K;
-          const uint32_t dst = ring + (uint32_t)(step % kShrinkStages * S::LOADS * 512);
+          const int k = step * kShrinkK;
+          const bool in = k + cc * 8 < pr.K;   // K ends inside the step: zeros from there on
+          const uint32_t to = (uint32_t)(stage * S::STAGE_ROWS * 128);
+          const __nv_bfloat16* src = in ? xp + k : pr.X;
+          const int64_t dx = in ? x4 : 0, da = in ? a4 : 0;
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int i = 0; i < S::ROWS / 4; ++i, src += dx)
+            if (wanted >> i & 1u) cp_async_16(dst_of[i & 1] + to + i * 512, src, in);
+          src = in ? ap + k : pr.A;
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const bool x_in = in && mine[mt][h];
-              cp_async_16(dst + (mt * 2 + h) * 512, x_in ? xp + (int64_t)(mt * 16 + h * 8) * pr.ldx + k : pr.X, x_in);
-            }
-#pragma unroll
-          for (int nt = 0; nt < NT8; ++nt) {
-            const bool a_in = in && nt * 8 < ranks_left;
-            cp_async_16(dst + (2 * MT + nt) * 512, a_in ? ap + (int64_t)(nt * 8) * pr.lda + k : pr.A, a_in);
-          }
+          for (int i = 0; i < S::COLS / 4; ++i, src += da)
+            if (i * 4 < ranks_left) cp_async_16(dst_of[i & 1] + to + S::ROWS * 128 + i * 512, src, in);
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
       };
+      load(step0, 0);
+      int stage = 0;
+      for (int step = step0; step < step1; step += by_k, stage ^= 1) {
+        load(step + by_k, stage ^ 1);   // into the stage that every lane is done with: the barrier at the end of the last round
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        __syncwarp();
+        const uint32_t src = ring + (uint32_t)(stage * S::STAGE_ROWS * 128 + g * 128);
+        uint4 w[2][NT8];
+        const uint32_t unit[2] = {(uint32_t)(q ^ shrink_swizzle(g)) << 4, (uint32_t)((4 + q) ^ shrink_swizzle(g)) << 4};   // every row read is g mod 8
 #pragma unroll
-      for (int i = 0; i < kShrinkStages - 1; ++i) load(step0 + i);
-      for (int step = step0; step < step1; ++step) {
-        load(step + kShrinkStages - 1);   // into the slot this lane read two steps ago
-        asm volatile("cp.async.wait_group %0;" ::"n"(kShrinkStages - 1) : "memory");
-        const uint32_t src = ring + (uint32_t)(step % kShrinkStages * S::LOADS * 512);
-        uint4 w[NT8];
+        for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int nt = 0; nt < NT8; ++nt) w[nt] = ld_shared_16(src + (2 * MT + nt) * 512);
+          for (int nt = 0; nt < NT8; ++nt) w[half][nt] = ld_shared_16(src + (S::ROWS + nt * 8) * 128 + unit[half]);
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
-          const uint4 x0 = ld_shared_16(src + (mt * 2) * 512), x1 = ld_shared_16(src + (mt * 2 + 1) * 512);
+          uint4 x[2][2];
 #pragma unroll
-          for (int nt = 0; nt < NT8; ++nt) {
-            // 32 k at a time in the tensor cores (which cut off low bits of a long running sum), added up in FP32
-            float t[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_m16n8k16_bf16(t, x0.x, x1.x, x0.y, x1.y, w[nt].x, w[nt].y);
-            mma_m16n8k16_bf16(t, x0.z, x1.z, x0.w, x1.w, w[nt].z, w[nt].w);
+          for (int half = 0; half < 2; ++half)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[mt][nt][e] += t[e];
-          }
+            for (int h = 0; h < 2; ++h) x[half][h] = ld_shared_16(src + mt * 2048 + h * 1024 + unit[half]);
+          // 64 k at a time in the tensor cores (which cut off low bits of a long running sum), added up in FP32
+          float t[NT8][4];
+#pragma unroll
+          for (int nt = 0; nt < NT8; ++nt)
+            mma_m16n8k16_bf16_zero(t[nt], x[0][0].x, x[0][1].x, x[0][0].y, x[0][1].y, w[0][nt].x, w[0][nt].y);
+#pragma unroll
+          for (int nt = 0; nt < NT8; ++nt) mma_m16n8k16_bf16(t[nt], x[0][0].z, x[0][1].z, x[0][0].w, x[0][1].w, w[0][nt].z, w[0][nt].w);
+#pragma unroll
+          for (int nt = 0; nt < NT8; ++nt) mma_m16n8k16_bf16(t[nt], x[1][0].x, x[1][1].x, x[1][0].y, x[1][1].y, w[1][nt].x, w[1][nt].y);
+#pragma unroll
+          for (int nt = 0; nt < NT8; ++nt) mma_m16n8k16_bf16(t[nt], x[1][0].z, x[1][1].z, x[1][0].w, x[1][1].w, w[1][nt].z, w[1][nt].w);
+#pragma unroll
+          for (int nt = 0; nt < NT8; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[mt][nt][e] += t[nt][e];
         }
+        __syncwarp();
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
+      __syncwarp();
     }
+    float* sums = slots <= kShrinkWarps ? warp_sums : block_sums;
+    const int ld = slots <= kShrinkWarps ? S::LD : S::COLS;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int lr = mt * 16 + h * 8 + g;
-        if (mine[mt][h]) {
+        if (__shfl_sync(0xffffffffu, ids.id[(mt * 16 + h * 8) / 32], lr % 32) == a) {
           if (q == 0) slot_of[lr] = slot;   // the same value from every warp that writes it
-          float* dst = warp_sums + (warp * S::ROWS + lr) * S::LD + 2 * q;
+          float* dst = sums + lr * ld + 2 * q;
 #pragma unroll
           for (int nt = 0; nt < NT8; ++nt)
             *reinterpret_cast<float2*>(dst + nt * 8) = make_float2(acc[mt][nt][2 * h], acc[mt][nt][2 * h + 1]);
@@ -203,12 +233,15 @@ lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
   }
   __syncthreads();
   const int elems = (row_end - row0) * S::COLS;
-  for (int e = threadIdx.x; e < elems; e += 32 * kShrinkWarps) {
-    const int lr = e / S::COLS, c = e % S::COLS;
-    if (id_of[lr] < 0) continue;
-    float sum = 0.f;
-    for (int w = slot_of[lr] % by_slot; w < kShrinkWarps; w += by_slot) sum += warp_sums[(w * S::ROWS + lr) * S::LD + c];
-    block_sums[e] = sum;
+  if (slots <= kShrinkWarps) {
+    for (int e = threadIdx.x; e < elems; e += 32 * kShrinkWarps) {
+      const int lr = e / S::COLS, c = e % S::COLS;
+      if (id_of[lr] < 0) continue;
+      float sum = 0.f;
+      for (int w = slot_of[lr] % by_slot; w < kShrinkWarps; w += by_slot)
+        sum += reinterpret_cast<const float*>(shrink_smem + w * S::RING_BYTES)[lr * S::LD + c];
+      block_sums[e] = sum;
+    }
   }
   __syncthreads();
   if (ranks > 1) {
@@ -429,24 +462,34 @@ lora_grad_kernel(const __grid_constant__ GradArgs args) {
 #pragma unroll
       for (int h = 0; h < 2; ++h)
         ldmatrix_x4_trans(b[k][h], qs + (k * 16 + (lane & 15)) * S::Q_PITCH + (warp_c + h * 16 + (lane >> 4) * 8) * 2);
+    // a step's products in the tensor cores (which cut off low bits of a long running sum), added up in FP32;
+    // two tiles of ranks at a time, so that eight chains of products are under way
+    constexpr int G = MT > 1 ? 2 : 1;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-      // a step's products in the tensor cores (which cut off low bits of a long running sum), added up in FP32
-      float tmp[4][4] = {};
+    for (int m0 = 0; m0 < MT; m0 += G) {
+      float tmp[G][4][4];
 #pragma unroll
       for (int t = TERMS - 1; t >= 0; --t)
 #pragma unroll
-        for (int k = 0; k < kGradTokens / 16; ++k) {
-          uint32_t r[4];    // P^T: 16 ranks x 16 tokens; matrices (tokens 0-7, 8-15) x (ranks 0-7, 8-15)
-          ldmatrix_x4_trans(r, ps + (k * 16 + (lane >> 4) * 8 + (lane & 7)) * S::P_PITCH + (t * S::RP + mt * 16 + ((lane >> 3) & 1) * 8) * 2);
+        for (int k = 0; k < kGradTokens / 16; ++k)
 #pragma unroll
-          for (int nt = 0; nt < 4; ++nt)
-            mma_m16n8k16_bf16(tmp[nt], r[0], r[1], r[2], r[3], b[k][nt >> 1][(nt & 1) * 2], b[k][nt >> 1][(nt & 1) * 2 + 1]);
-        }
+          for (int m = 0; m < G; ++m) {
+            uint32_t r[4];    // P^T: 16 ranks x 16 tokens; matrices (tokens 0-7, 8-15) x (ranks 0-7, 8-15)
+            ldmatrix_x4_trans(r, ps + (k * 16 + (lane >> 4) * 8 + (lane & 7)) * S::P_PITCH + (t * S::RP + (m0 + m) * 16 + ((lane >> 3) & 1) * 8) * 2);
 #pragma unroll
-      for (int nt = 0; nt < 4; ++nt)
+            for (int nt = 0; nt < 4; ++nt) {
+              if (t == TERMS - 1 && k == 0)
+                mma_m16n8k16_bf16_zero(tmp[m][nt], r[0], r[1], r[2], r[3], b[k][nt >> 1][(nt & 1) * 2], b[k][nt >> 1][(nt & 1) * 2 + 1]);
+              else
+                mma_m16n8k16_bf16(tmp[m][nt], r[0], r[1], r[2], r[3], b[k][nt >> 1][(nt & 1) * 2], b[k][nt >> 1][(nt & 1) * 2 + 1]);
+            }
+          }
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[mt][nt][e] += tmp[nt][e];
+      for (int m = 0; m < G; ++m)
+#pragma unroll
+        for (int nt = 0; nt < 4; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) acc[m0 + m][nt][e] += tmp[m][nt][e];
     }
     if (warp == 0) row_ring[(it + kGradStages) % kGradRows][lane] = next_row;
     cu.pos += min(kGradTokens, cu.end - cu.pos);

@@ -353,6 +353,11 @@ static int launch_splitk_reduce(const float* scratch, int64_t M, int64_t N, int 
   return GEMM_B200_OK;
 }
 
+// A product whose A has fewer rows than this streams B slowly: the loads of 128-row boxes with fewer than 16
+// rows inside the matrix hold up the ring (131072 x 4096 bf16 B, 128-column tiles: 1 row 239 us, 15 rows 233,
+// 16 rows 166, 64 rows 169).  Operators with scratch of their own give A that many rows.
+constexpr int64_t kMinMapRows = 16;
+
 struct Bf16Args {
   const void *A, *B;
   void* C;
@@ -362,6 +367,8 @@ struct Bf16Args {
   int64_t batch = 1, stride_a = 0, stride_b = 0, stride_c = 0;
   // split-K (FP32 output only): C is then the scratch [k_splits][M][N], ldc = N
   int k_splits = 1;
+  // rows of A in memory where there are more than M (plain layout, one problem; see kMinMapRows); 0: M
+  int64_t a_rows = 0;
 };
 
 // One instantiation per (config, B layout, output type); A_MN: A is stored transposed, [K, M] row-major;
@@ -382,8 +389,8 @@ static int launch_bf16_fused(const Bf16Args& a, const Fuse& fuse) {
                              CU_TENSOR_MAP_SWIZZLE_128B))
       return rc;
   } else {
-    if (int rc = make_map_3d(&tmA, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.A, a.M, a.K, a.lda, za, sa, kBlockK, kBlockM,
-                             CU_TENSOR_MAP_SWIZZLE_128B))
+    if (int rc = make_map_3d(&tmA, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.A, a.a_rows ? a.a_rows : a.M, a.K, a.lda, za,
+                             a.a_rows ? a.a_rows * a.lda : sa, kBlockK, kBlockM, CU_TENSOR_MAP_SWIZZLE_128B))
       return rc;
   }
   if (B_MN) {

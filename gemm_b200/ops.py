@@ -252,23 +252,60 @@ def gemm_bf16_grouped(A: torch.Tensor, B: torch.Tensor, m_sizes, out: torch.Tens
     return out
 
 
+# The operators below take eight tensors and more: their checks read every attribute once, and a message is put
+# together only for the error it belongs to (10 us of a call that takes 20 on the device).
 def _vector(t: torch.Tensor, n: int, dtype: torch.dtype, device: torch.device, name: str, strided: bool = False) -> None:
-    _require(t.device == device and t.dtype == dtype and t.dim() == 1 and t.shape[0] == n and (strided or n <= 1 or t.stride(0) == 1),
-             f"{name} must be a {'' if strided else 'contiguous '}1-D {dtype} tensor of {n} elements on {device}")
+    if t.device != device or t.dtype != dtype or t.shape != (n,) or not (strided or n <= 1 or t.stride(0) == 1):
+        raise ValueError(f"{name} must be a {'' if strided else 'contiguous '}1-D {dtype} tensor of {n} elements on {device}")
+
+
+def _matrix(t: torch.Tensor, device: torch.device, name: str) -> tuple[int, int, int]:
+    """(rows, columns, row pitch) of a row-major 2-D bfloat16 tensor."""
+    if t.device != device or t.dtype != torch.bfloat16 or t.dim() != 2:
+        raise ValueError(f"{name} must be a 2-D bfloat16 tensor on {device}")
+    (rows, cols), (ld, one) = t.shape, t.stride()
+    if one != 1 and cols > 1:
+        raise ValueError(f"{name} must be row-major (unit column stride)")
+    return rows, cols, ld if rows > 1 else max(cols, 1)
+
+
+def _stack(t: torch.Tensor, device: torch.device, name: str) -> tuple[int, int, int, int, int]:
+    """(matrices, rows, columns, row pitch, matrix stride) of a 3-D bfloat16 tensor of row-major matrices."""
+    if t.device != device or t.dtype != torch.bfloat16 or t.dim() != 3:
+        raise ValueError(f"{name} must be a 3-D bfloat16 tensor on {device}")
+    (n, rows, cols), (stride, ld, one) = t.shape, t.stride()
+    if one != 1 and cols > 1:
+        raise ValueError(f"the last dimension of {name} must be contiguous")
+    if rows <= 1:
+        ld = max(cols, 1)
+    return n, rows, cols, ld, stride if n > 1 else rows * ld   # the stride of a dimension of one element means nothing
+
+
+def _out_matrix(t: torch.Tensor, device: torch.device, dtype: torch.dtype, rows: int, cols: int) -> int:
+    if t.device != device or t.dtype != dtype or t.shape != (rows, cols):
+        raise ValueError(f"bad out tensor: expected {dtype} {(rows, cols)} on {device}")
+    return _row_major_ld(t)
 
 
 def _scratch(nbytes: int, device: torch.device) -> torch.Tensor:
     # from torch's allocator, per call: private to the call's stream, and to the graph a capture makes
-    return torch.empty((max(int(nbytes), 1),), device=device, dtype=torch.uint8)
+    return torch.empty(nbytes or 1, device=device, dtype=torch.uint8)
 
 
-def _xent_operands(X: torch.Tensor, W: torch.Tensor, labels: torch.Tensor) -> tuple[int, int, int]:
-    _require(X.is_cuda and W.device == X.device, "X and W must be CUDA tensors on one device")
-    _require(X.dtype == torch.bfloat16 and W.dtype == torch.bfloat16, "expected bfloat16")
-    _require(X.dim() == 2 and W.dim() == 2 and X.shape[1] == W.shape[1], f"X is {tuple(X.shape)} but W is {tuple(W.shape)}")
-    T, D = X.shape
-    _vector(labels, T, torch.int64, X.device, "labels")
-    return T, W.shape[0], D
+def _cuda_device(X: torch.Tensor) -> torch.device:
+    if not X.is_cuda:
+        raise ValueError("expected CUDA tensors")
+    return X.device
+
+
+def _xent_operands(X: torch.Tensor, W: torch.Tensor, labels: torch.Tensor):
+    device = _cuda_device(X)
+    T, D, ldx = _matrix(X, device, "X")
+    V, Dw, ldw = _matrix(W, device, "W")
+    if D != Dw:
+        raise ValueError(f"X is {tuple(X.shape)} but W is {tuple(W.shape)}")
+    _vector(labels, T, torch.int64, device, "labels")
+    return device, T, V, D, ldx, ldw
 
 
 def gemm_bf16_xent(X: torch.Tensor, W: torch.Tensor, labels: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
@@ -277,14 +314,13 @@ def gemm_bf16_xent(X: torch.Tensor, W: torch.Tensor, labels: torch.Tensor) -> tu
     ``X`` is ``[T, D]``, ``W`` the vocabulary projection ``[V, D]``, ``labels`` int64 ``[T]``;
     ``lse[t] = log(sum_v exp(logit[t, v]))`` and ``loss[t] = lse[t] - logit[t, labels[t]]``.  A negative label
     (padding) has loss 0; a label >= V makes its loss NaN.  Logits, maxima and sums are FP32."""
-    T, V, D = _xent_operands(X, W, labels)
-    loss = torch.empty((T,), device=X.device, dtype=torch.float32)
-    lse = torch.empty((T,), device=X.device, dtype=torch.float32)
-    nbytes = lib.gemm_b200_gemm_bf16_xent_scratch_bytes(T, V)
-    scratch = _scratch(nbytes, X.device)
-    with _OnDevice(X.device):
-        check(lib.gemm_b200_gemm_bf16_xent(X.data_ptr(), W.data_ptr(), labels.data_ptr(), loss.data_ptr(), lse.data_ptr(), T, V, D,
-                                           _row_major_ld(X), _row_major_ld(W), scratch.data_ptr(), nbytes, _stream(X)))
+    device, T, V, D, ldx, ldw = _xent_operands(X, W, labels)
+    loss, lse = torch.empty((2, T), device=device, dtype=torch.float32)
+    nbytes = lib.gemm_b200_gemm_bf16_xent_scratch_bytes(T, V, D)
+    scratch = _scratch(nbytes, device)
+    with _OnDevice(device):
+        check(lib.gemm_b200_gemm_bf16_xent(X.data_ptr(), W.data_ptr(), labels.data_ptr(), loss.data_ptr(), lse.data_ptr(), T, V, D, ldx, ldw,
+                                           scratch.data_ptr(), nbytes, _stream(X)))
     return loss, lse
 
 
@@ -298,44 +334,40 @@ def gemm_bf16_xent_grad(X: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, 
     vocabulary at a time.  A row whose gradients are zero, as padding's are, adds nothing to ``dW`` whatever
     its ``X`` holds.  ``grad_loss`` is not read where the label is negative; a label >= V makes its
     row of ``dX``, and ``dW``, NaN."""
-    T, V, D = _xent_operands(X, W, labels)
-    _vector(lse, T, torch.float32, X.device, "lse")
-    _vector(grad_loss, T, torch.float32, X.device, "grad_loss", strided=True)
+    device, T, V, D, ldx, ldw = _xent_operands(X, W, labels)
+    _vector(lse, T, torch.float32, device, "lse")
+    _vector(grad_loss, T, torch.float32, device, "grad_loss", strided=True)
+    h, h_stride = 0, 0
     if grad_lse is not None:
-        _vector(grad_lse, T, torch.float32, X.device, "grad_lse", strided=True)
+        _vector(grad_lse, T, torch.float32, device, "grad_lse", strided=True)
+        h, h_stride = grad_lse.data_ptr(), grad_lse.stride(0)
     if out is None:
-        dX = torch.empty((T, D), device=X.device, dtype=torch.bfloat16)
-        dW = torch.empty((V, D), device=X.device, dtype=torch.bfloat16)
+        dX = torch.empty((T, D), device=device, dtype=torch.bfloat16)
+        dW = torch.empty((V, D), device=device, dtype=torch.bfloat16)
+        lddx = lddw = D
     else:
         dX, dW = out
-        for t, rows in ((dX, T), (dW, V)):
-            _require(t.device == X.device and t.dtype == torch.bfloat16 and tuple(t.shape) == (rows, D), "bad out tensor")
-    with _OnDevice(X.device):
+        lddx, lddw = _out_matrix(dX, device, torch.bfloat16, T, D), _out_matrix(dW, device, torch.bfloat16, V, D)
+    with _OnDevice(device):
         nbytes = lib.gemm_b200_gemm_bf16_xent_grad_scratch_bytes(T, V, D)
-        scratch = _scratch(nbytes, X.device)
+        scratch = _scratch(nbytes, device)
         check(lib.gemm_b200_gemm_bf16_xent_grad(
-            X.data_ptr(), W.data_ptr(), labels.data_ptr(), lse.data_ptr(), grad_loss.data_ptr(), grad_loss.stride(0),
-            0 if grad_lse is None else grad_lse.data_ptr(), 0 if grad_lse is None else grad_lse.stride(0), dX.data_ptr(), dW.data_ptr(),
-            T, V, D, _row_major_ld(X), _row_major_ld(W), _row_major_ld(dX), _row_major_ld(dW), scratch.data_ptr(), nbytes, _stream(X)))
+            X.data_ptr(), W.data_ptr(), labels.data_ptr(), lse.data_ptr(), grad_loss.data_ptr(), grad_loss.stride(0), h, h_stride,
+            dX.data_ptr(), dW.data_ptr(), T, V, D, ldx, ldw, lddx, lddw, scratch.data_ptr(), nbytes, _stream(X)))
     return dX, dW
 
 
-def _lora_operands(X, A, B, ids, scales, N: int) -> tuple[int, int, int, int, int, int, int, int]:
-    _require(X.is_cuda and A.device == X.device and B.device == X.device, "X, A and B must be CUDA tensors on one device")
-    _require(X.dtype == torch.bfloat16 and A.dtype == torch.bfloat16 and B.dtype == torch.bfloat16, "expected bfloat16")
-    _require(X.dim() == 2 and A.dim() == 3 and B.dim() == 3, "X must be 2-D, A and B 3-D")
-    T, D = X.shape
-    n, R = A.shape[0], A.shape[1]
-    _require(A.shape[2] == D and B.shape[0] == n and B.shape[1] == R and B.shape[2] == N,
-             f"X is {tuple(X.shape)}, A {tuple(A.shape)}, B {tuple(B.shape)}, and the projection has {N} columns")
-    _vector(ids, T, torch.int32, X.device, "ids")
-    if scales is not None:
-        _vector(scales, n, torch.float32, X.device, "scales")
-    lda, sa = _batch_layout(A)
-    ldb, sb = _batch_layout(B)
-    if n == 1:   # the stride of a dimension of one element means nothing
-        sa, sb = R * lda, R * ldb
-    return T, D, n, R, lda, sa, ldb, sb
+def _lora_adapters(A, B, ids, scales, device, T: int, D: int, N: int):
+    """(n, R, lda, stride_a, ldb, stride_b, address of scales) of checked adapters."""
+    n, R, Da, lda, sa = _stack(A, device, "A")
+    nb, Rb, Nb, ldb, sb = _stack(B, device, "B")
+    if nb != n or Rb != R or Da != D or Nb != N:
+        raise ValueError(f"A is {tuple(A.shape)} and B {tuple(B.shape)}, but the projection is {D} x {N}")
+    _vector(ids, T, torch.int32, device, "ids")
+    if scales is None:
+        return n, R, lda, sa, ldb, sb, 0
+    _vector(scales, n, torch.float32, device, "scales")
+    return n, R, lda, sa, ldb, sb, scales.data_ptr()
 
 
 def gemm_bf16_lora(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.Tensor, ids: torch.Tensor,
@@ -349,22 +381,28 @@ def gemm_bf16_lora(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.T
     means no adapter; ``scales`` is FP32 ``[n]``.  An id >= n makes its row NaN.  Rows of one adapter are
     cheapest next to each other.  The gradient with respect to X is the same operator,
     ``gemm_bf16_lora(dY, W, B, A, ids, scales, b_is_nk=not b_is_nk)``."""
-    _require(W.device == X.device and W.dtype == torch.bfloat16 and W.dim() == 2, "W must be a 2-D CUDA bfloat16 tensor")
-    _require(out_dtype in (torch.bfloat16, torch.float32), "out_dtype must be bfloat16 or float32")
-    N = W.shape[0] if b_is_nk else W.shape[1]
-    T, D, n, R, lda, sa, ldb, sb = _lora_operands(X, A, B, ids, scales, N)
-    _require(W.shape[1 if b_is_nk else 0] == D, f"X is {tuple(X.shape)} but W is {tuple(W.shape)}")
+    device = _cuda_device(X)
+    T, D, ldx = _matrix(X, device, "X")
+    K, N, ldw = _matrix(W, device, "W")
+    if b_is_nk:
+        K, N = N, K
+    if K != D:
+        raise ValueError(f"X is {tuple(X.shape)} but W is {tuple(W.shape)}")
+    n, R, lda, sa, ldb, sb, scale_ptr = _lora_adapters(A, B, ids, scales, device, T, D, N)
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("out_dtype must be bfloat16 or float32")
     if out is None:
-        out = torch.empty((T, N), device=X.device, dtype=out_dtype)
-    _require(out.device == X.device and out.dtype == out_dtype and tuple(out.shape) == (T, N), "bad out tensor")
+        out = torch.empty((T, N), device=device, dtype=out_dtype)
+        ldy = N
+    else:
+        ldy = _out_matrix(out, device, out_dtype, T, N)
     od = _lib.OUT_F32 if out_dtype == torch.float32 else _lib.OUT_BF16
-    with _OnDevice(X.device):
+    with _OnDevice(device):
         nbytes = lib.gemm_b200_gemm_bf16_lora_scratch_bytes(T, N, D, R, od)
-        scratch = _scratch(nbytes, X.device)
+        scratch = _scratch(nbytes, device)
         check(lib.gemm_b200_gemm_bf16_lora(
-            X.data_ptr(), W.data_ptr(), A.data_ptr(), B.data_ptr(), ids.data_ptr(), 0 if scales is None else scales.data_ptr(),
-            out.data_ptr(), T, N, D, R, n, _row_major_ld(X), _row_major_ld(W), lda, sa, ldb, sb, _row_major_ld(out),
-            _lib.B_ROW_MAJOR_NK if b_is_nk else _lib.B_ROW_MAJOR_KN, od, scratch.data_ptr(), nbytes, _stream(X)))
+            X.data_ptr(), W.data_ptr(), A.data_ptr(), B.data_ptr(), ids.data_ptr(), scale_ptr, out.data_ptr(), T, N, D, R, n, ldx, ldw, lda, sa,
+            ldb, sb, ldy, _lib.B_ROW_MAJOR_NK if b_is_nk else _lib.B_ROW_MAJOR_KN, od, scratch.data_ptr(), nbytes, _stream(X)))
     return out
 
 
@@ -374,26 +412,29 @@ def gemm_bf16_lora_grad(X: torch.Tensor, dY: torch.Tensor, A: torch.Tensor, B: t
     """Gradients of the adapters of ``gemm_bf16_lora``: ``(dA, dB)``, contiguous ``[n, R, D]`` and ``[n, R, N]`` in bfloat16 or
     FP32, for the output gradient ``dY`` ``[T, N]``.  Rows with an id outside [0, n) add nothing; adapters without a
     row get zeros.  The order of every sum is fixed."""
-    _require(dY.device == X.device and dY.dtype == torch.bfloat16 and dY.dim() == 2 and dY.shape[0] == X.shape[0],
-             "dY must be a 2-D CUDA bfloat16 tensor with the rows of X")
-    _require(out_dtype in (torch.bfloat16, torch.float32), "out_dtype must be bfloat16 or float32")
-    N = dY.shape[1]
-    T, D, n, R, lda, sa, ldb, sb = _lora_operands(X, A, B, ids, scales, N)
+    device = _cuda_device(X)
+    T, D, ldx = _matrix(X, device, "X")
+    Ty, N, lddy = _matrix(dY, device, "dY")
+    if Ty != T:
+        raise ValueError(f"X is {tuple(X.shape)} but dY is {tuple(dY.shape)}")
+    n, R, lda, sa, ldb, sb, scale_ptr = _lora_adapters(A, B, ids, scales, device, T, D, N)
+    if out_dtype not in (torch.bfloat16, torch.float32):
+        raise ValueError("out_dtype must be bfloat16 or float32")
     if out is None:
-        dA = torch.empty((n, R, D), device=X.device, dtype=out_dtype)
-        dB = torch.empty((n, R, N), device=X.device, dtype=out_dtype)
+        dA = torch.empty((n, R, D), device=device, dtype=out_dtype)
+        dB = torch.empty((n, R, N), device=device, dtype=out_dtype)
     else:
         dA, dB = out
         for t, like in ((dA, A), (dB, B)):
-            _require(t.device == X.device and t.dtype == out_dtype and t.shape == like.shape and t.is_contiguous(), "bad out tensor")
+            if t.device != device or t.dtype != out_dtype or t.shape != like.shape or not t.is_contiguous():
+                raise ValueError(f"bad out tensor: expected a contiguous {out_dtype} tensor {tuple(like.shape)} on {device}")
     od = _lib.OUT_F32 if out_dtype == torch.float32 else _lib.OUT_BF16
-    with _OnDevice(X.device):
+    with _OnDevice(device):
         nbytes = lib.gemm_b200_gemm_bf16_lora_grad_scratch_bytes(T, N, D, R, n, od)
-        scratch = _scratch(nbytes, X.device)
+        scratch = _scratch(nbytes, device)
         check(lib.gemm_b200_gemm_bf16_lora_grad(
-            X.data_ptr(), dY.data_ptr(), A.data_ptr(), B.data_ptr(), ids.data_ptr(), 0 if scales is None else scales.data_ptr(),
-            dA.data_ptr(), dB.data_ptr(), T, N, D, R, n, _row_major_ld(X), _row_major_ld(dY), lda, sa, ldb, sb, od,
-            scratch.data_ptr(), nbytes, _stream(X)))
+            X.data_ptr(), dY.data_ptr(), A.data_ptr(), B.data_ptr(), ids.data_ptr(), scale_ptr, dA.data_ptr(), dB.data_ptr(), T, N, D, R, n, ldx,
+            lddy, lda, sa, ldb, sb, od, scratch.data_ptr(), nbytes, _stream(X)))
     return dA, dB
 
 

@@ -188,7 +188,7 @@ int gemm_b200_gemm_bf16_grouped(const void* A, const void* B, void* C, int64_t g
 int gemm_b200_gemm_bf16_xent(const void* X, const void* W, const int64_t* labels, float* loss, float* lse,
                              int64_t T, int64_t V, int64_t D, int64_t ldx, int64_t ldw,
                              void* scratch, size_t scratch_bytes, void* stream);
-size_t gemm_b200_gemm_bf16_xent_scratch_bytes(int64_t T, int64_t V);
+size_t gemm_b200_gemm_bf16_xent_scratch_bytes(int64_t T, int64_t V, int64_t D);
 
 /* Its gradient, with lse as the call above wrote it:
  *   d_tv = (g_t + h_t) exp(z_tv - lse_t) - g_t [v == labels[t]],   dX = d W,   dW = d^T X   (bf16)
