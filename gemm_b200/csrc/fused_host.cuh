@@ -431,15 +431,29 @@ static int lora_entry(const void* X, const void* W, const void* A, const void* B
                       : launch_lora<Bf16_2cta_tma_m, false>(a, fuse, w_layout);
 }
 
+static int lora_grad_per_sm(int rp, int terms) {
+  if (terms == 1)
+    return rp == 16 ? GradShape<1, 1>::PER_SM : rp == 32 ? GradShape<2, 1>::PER_SM : rp == 64 ? GradShape<4, 1>::PER_SM : GradShape<8, 1>::PER_SM;
+  return rp == 16 ? GradShape<1, 3>::PER_SM : rp == 32 ? GradShape<2, 3>::PER_SM : rp == 64 ? GradShape<4, 3>::PER_SM : GradShape<8, 3>::PER_SM;
+}
+
 struct LoraGradPlan {
   int64_t chunks_d, chunks_n, block_tokens, blocks;
-  LoraGradPlan(int64_t T, int64_t N, int64_t D, int sms) {
+  LoraGradPlan(int64_t T, int64_t N, int64_t D, int64_t R, int terms, int sms) {
     chunks_d = ceil_div64(D, kGradCols);
     chunks_n = ceil_div64(N, kGradCols);
-    // blocks of tokens until about four thread blocks per SM are there, but not below 64 tokens
-    int64_t want = ceil_div64(4 * (int64_t)sms, chunks_d + chunks_n);
-    const int64_t most = ceil_div64(T, 64);
-    if (want > most) want = most;
+    // Blocks of tokens so that the grid fills one, two or three rounds of the resident thread blocks best (672 thread
+    // blocks on 444 places: a third of the second round idle), but not below 64 tokens.
+    const int64_t chunks = chunks_d + chunks_n, slots = (int64_t)sms * lora_grad_per_sm(lora_rp(R), terms), most = ceil_div64(T, 64);
+    int64_t want = 1;
+    double best = 0;
+    for (int rounds = 1; rounds <= 3; ++rounds) {
+      int64_t b = rounds * slots / chunks;
+      if (b < 1) b = 1;
+      if (b > most) b = most;
+      const double fill = (double)(b * chunks) / (double)(ceil_div64(b * chunks, slots) * slots);
+      if (fill > best + 0.03) { best = fill; want = b; }
+    }
     if (want < 1) want = 1;
     block_tokens = ceil_div64(ceil_div64(T > 0 ? T : 1, want), kGradTokens) * kGradTokens;
     blocks = ceil_div64(T > 0 ? T : 1, block_tokens);
@@ -496,8 +510,8 @@ static int lora_grad_entry(const void* X, const void* dY, const void* A, const v
   }
   DeviceInfo di;
   if (int rc = check_blackwell("gemm_bf16_lora_grad", &di)) return rc;
-  const LoraGradPlan plan(T, N, D, di.sms);
   const int terms = lora_terms(out_dtype), rp = lora_rp(R);
+  const LoraGradPlan plan(T, N, D, R, terms, di.sms);
   const LoraGradScratch ws(scratch, T, N, D, R, n, terms, plan);
   if (int rc = check_scratch("gemm_bf16_lora_grad", scratch, scratch_bytes, ws.bytes)) return rc;
 
@@ -575,7 +589,7 @@ extern "C" size_t gemm_b200_gemm_bf16_lora_grad_scratch_bytes(int64_t T, int64_t
   using namespace gemm_b200::tc;
   const int sms = current_sms();
   if (T <= 0 || N <= 0 || D <= 0 || R <= 0 || R > kLoraMaxRank || adapters <= 0 || sms <= 0) return 0;
-  return LoraGradScratch(nullptr, T, N, D, R, adapters, lora_terms(out_dtype), LoraGradPlan(T, N, D, sms)).bytes;
+  return LoraGradScratch(nullptr, T, N, D, R, adapters, lora_terms(out_dtype), LoraGradPlan(T, N, D, R, lora_terms(out_dtype), sms)).bytes;
 }
 extern "C" int gemm_b200_gemm_bf16_lora_grad(const void* X, const void* dY, const void* A, const void* B, const int32_t* ids,
                                              const float* scales, void* dA, void* dB, int64_t T, int64_t N, int64_t D, int64_t R,

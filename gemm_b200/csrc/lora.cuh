@@ -350,7 +350,7 @@ struct GradArgs {
   const int32_t* start;
   int n, R, block_tokens;
 };
-constexpr int kGradCols = 128, kGradTokens = 32, kGradStages = 4, kGradThreads = 128;
+constexpr int kGradCols = 128, kGradTokens = 32, kGradStages = 3, kGradThreads = 128;
 constexpr int kGradRows = 8;   // steps whose row indices are held: more than the stages, so that no reader is overtaken
 
 template <int MT, int TERMS>
@@ -359,6 +359,9 @@ struct GradShape {
   static constexpr int Q_PITCH = kGradCols * 2 + 16, P_PITCH = RP * TERMS * 2 + 16;   // odd multiples of 16 bytes: ldmatrix without conflicts
   static constexpr int STAGE_BYTES = kGradTokens * (Q_PITCH + P_PITCH);
   static constexpr int SMEM_BYTES = kGradStages * STAGE_BYTES;
+  // blocks per SM by shared memory and by registers (80, 128, 168, 255 a thread for 16, 32, 64, 128 ranks)
+  static constexpr int BY_SMEM = 231424 / (SMEM_BYTES + 1536), BY_REGS = MT == 1 ? 6 : MT == 2 ? 4 : MT == 4 ? 3 : 2;
+  static constexpr int PER_SM = BY_SMEM < BY_REGS ? BY_SMEM : BY_REGS;
 };
 
 // Walks the steps of one block: positions [pos, end) of adapter a, at most 32 at a time.
@@ -408,25 +411,28 @@ lora_grad_kernel(const __grid_constant__ GradArgs args) {
     ix.settle(args.start, args.n);
     return row;
   };
+  // sixteen threads per token, eight tokens at a time: a thread keeps its columns, so that a copy costs it a row
+  // index, one multiplication and the instruction itself
+  const int t0 = threadIdx.x / 16, piece = threadIdx.x % 16;
+  const bool col_in = c0 + piece * 8 < pr.cols;
+  const __nv_bfloat16* q_src = col_in ? pr.Q + c0 + piece * 8 : pr.Q;
+  const uint32_t q_dst = (uint32_t)(t0 * S::Q_PITCH + piece * 16), p_dst = (uint32_t)(kGradTokens * S::Q_PITCH + t0 * S::P_PITCH + piece * 16);
+  constexpr int PIECES = S::RP * TERMS / 8;   // of a row of P
   auto load_step = [&](int step) {
     const int* rows = row_ring[step % kGradRows];
-    const uint32_t qs = smem + (step % kGradStages) * S::STAGE_BYTES, ps = qs + kGradTokens * S::Q_PITCH;
+    const uint32_t base = smem + (step % kGradStages) * S::STAGE_BYTES;
     if (rows[0] >= 0) {   // past the last step: an empty group
 #pragma unroll
-      for (int i = 0; i < kGradTokens * (kGradCols / 8) / kGradThreads; ++i) {
-        const int e = threadIdx.x + i * kGradThreads, t = e / (kGradCols / 8), c = e % (kGradCols / 8) * 8;
-        const int row = rows[t];
-        const bool in = row >= 0 && c0 + c < pr.cols;
-        cp_async_16(qs + t * S::Q_PITCH + c * 2, in ? pr.Q + row * pr.ldq + c0 + c : pr.Q, in);
-      }
-      constexpr int PV = S::RP * TERMS / 8;
+      for (int i = 0; i < kGradTokens / 8; ++i) {
+        const int row = rows[t0 + i * 8];
+        const bool in = row >= 0;
+        const int64_t at = in ? row : 0;
+        cp_async_16(base + q_dst + i * 8 * S::Q_PITCH, q_src + at * pr.ldq, in && col_in);
+        const __nv_bfloat16* p_src = pr.P + at * ldp + piece * 8;
 #pragma unroll
-      for (int i = 0; i < (kGradTokens * PV + kGradThreads - 1) / kGradThreads; ++i) {
-        const int e = threadIdx.x + i * kGradThreads, t = e / PV, c = e % PV * 8;
-        if (kGradTokens * PV % kGradThreads == 0 || e < kGradTokens * PV) {
-          const int row = rows[t];
-          cp_async_16(ps + t * S::P_PITCH + c * 2, row >= 0 ? pr.P + row * ldp + c : pr.P, row >= 0);
-        }
+        for (int j = 0; j < (PIECES + 15) / 16; ++j)
+          if (PIECES % 16 == 0 || j < PIECES / 16 || piece + j * 16 < PIECES)
+            cp_async_16(base + p_dst + i * 8 * S::P_PITCH + j * 256, p_src + j * 128, in);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
