@@ -313,34 +313,56 @@ static int lora_sizes(const char* who, int64_t T, int64_t N, int64_t D, int64_t 
   return GEMM_B200_OK;
 }
 
-template <int MT, int NT8>
-static int launch_shrink(ShrinkArgs args, int problems, int64_t max_k, const DeviceInfo& di, cudaStream_t st) {
-  using S = ShrinkShape<MT, NT8>;
-  auto kern = lora_shrink_kernel<MT, NT8>;
-  if (int rc = allow_smem(kern, S::SMEM_BYTES, di)) return rc;
-  const int64_t blocks = ceil_div64(args.T, args.rows_per_block);
-  // K over the blocks of a cluster until most SMs have one, as long as every warp keeps a step of 64 k
+// K over the blocks of a cluster until most SMs have one, as long as every block keeps a step of its eight warps.
+static int shrink_cluster(int64_t blocks, int64_t max_k, const DeviceInfo& di) {
   int ks = 1;
-  while (ks < kShrinkMaxCluster && 5 * blocks * problems * args.chunks * ks < 4 * (int64_t)di.sms && max_k / kShrinkK >= 2 * ks * kShrinkWarps) ks *= 2;
-  return launch_plain(kern, dim3((unsigned)blocks, (unsigned)ks, (unsigned)(problems * args.chunks)), 32 * kShrinkWarps, S::SMEM_BYTES, ks,
-                      st, args);
+  while (ks < kShrinkMaxCluster && 5 * blocks * ks < 4 * (int64_t)di.sms && max_k / (kShrinkK * kShrinkWarps) >= 2 * ks) ks *= 2;
+  return ks;
+}
+
+template <int NT8>
+static int launch_shrink_few(ShrinkArgs args, int problems, int64_t max_k, const DeviceInfo& di, cudaStream_t st) {
+  using S = ShrinkShape<1, NT8>;
+  auto kern = lora_shrink_kernel<1, NT8>;
+  if (int rc = allow_smem(kern, S::SMEM_BYTES, di)) return rc;
+  // a block per row, so that every adapter streams on its own; from 65 rows on 16 share a block
+  args.rows_per_block = args.T <= 64 ? 1 : S::ROWS;
+  const int64_t blocks = ceil_div64(args.T, args.rows_per_block), z = problems * args.chunks;
+  const int ks = shrink_cluster(blocks * z, max_k, di);
+  return launch_plain(kern, dim3((unsigned)blocks, (unsigned)ks, (unsigned)z), 32 * kShrinkWarps, S::SMEM_BYTES, ks, st, args);
+}
+
+template <int MT, int NT8>
+static int launch_shrink_rows(ShrinkArgs args, int problems, int64_t max_k, const DeviceInfo& di, cudaStream_t st) {
+  using S = ShrinkRowsShape<MT, NT8>;
+  auto kern = lora_shrink_rows_kernel<MT, NT8>;
+  if (int rc = allow_smem(kern, S::SMEM_BYTES, di)) return rc;
+  args.rows_per_block = S::ROWS;
+  ShrinkMaps maps;
+  for (int i = 0; i < 2; ++i) {
+    const ShrinkProblem& p = args.p[i < problems ? i : 0];
+    if (int rc = make_map_3d(&maps.x[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.X, args.T, p.K, p.ldx, 1, args.T * p.ldx, kShrinkK, S::ROWS,
+                             CU_TENSOR_MAP_SWIZZLE_128B))
+      return rc;
+    if (int rc = make_map_3d(&maps.a[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p.A, args.R, p.K, p.lda, args.n, p.stride_a, kShrinkK, S::COLS,
+                             CU_TENSOR_MAP_SWIZZLE_128B))
+      return rc;
+  }
+  const int64_t blocks = ceil_div64(args.T, S::ROWS), z = problems * args.chunks;
+  const int ks = shrink_cluster(blocks * z, max_k, di);
+  return launch_plain(kern, dim3((unsigned)blocks, (unsigned)ks, (unsigned)z), 32 * kShrinkWarps, S::SMEM_BYTES, ks, st, args, maps);
 }
 
 static int lora_shrink(ShrinkArgs args, int problems, int64_t max_k, const DeviceInfo& di, cudaStream_t st) {
   args.chunks = args.rp > 64 ? 2 : 1;
   const int cols = args.rp > 64 ? 64 : args.rp;
-  // few rows: a block per row, so that every adapter streams on its own; many rows: 32 or 64 rows share the
-  // adapter's fragments; between them 16
-  if (args.T < 512) {
-    args.rows_per_block = args.T <= 64 ? 1 : 16;
-    return cols == 16   ? launch_shrink<1, 2>(args, problems, max_k, di, st)
-           : cols == 32 ? launch_shrink<1, 4>(args, problems, max_k, di, st)
-                        : launch_shrink<1, 8>(args, problems, max_k, di, st);
-  }
-  args.rows_per_block = cols == 64 ? 32 : 64;
-  return cols == 16   ? launch_shrink<4, 2>(args, problems, max_k, di, st)
-         : cols == 32 ? launch_shrink<4, 4>(args, problems, max_k, di, st)
-                      : launch_shrink<2, 8>(args, problems, max_k, di, st);
+  if (args.T < 512)
+    return cols == 16   ? launch_shrink_few<2>(args, problems, max_k, di, st)
+           : cols == 32 ? launch_shrink_few<4>(args, problems, max_k, di, st)
+                        : launch_shrink_few<8>(args, problems, max_k, di, st);
+  return cols == 16   ? launch_shrink_rows<4, 2>(args, problems, max_k, di, st)
+         : cols == 32 ? launch_shrink_rows<4, 4>(args, problems, max_k, di, st)
+                      : launch_shrink_rows<2, 8>(args, problems, max_k, di, st);
 }
 
 struct LoraScratch {
@@ -526,6 +548,7 @@ static int lora_grad_entry(const void* X, const void* dY, const void* A, const v
   sa.n = (int)n;
   sa.rp = rp;
   sa.terms = terms;
+  sa.beside = true;
   if (int rc = lora_shrink(sa, 2, D > N ? D : N, di, st)) return rc;
 
   GradArgs ga = {};

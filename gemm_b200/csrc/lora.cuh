@@ -70,6 +70,9 @@ struct ShrinkArgs {
   const int32_t* ids;
   const float* scales;   // may be null: 1
   int T, R, n, rp, terms, rows_per_block, chunks;   // chunks of 64 ranks
+  // launched behind a kernel whose output is not read here (lora_sort_kernel, which lets it be scheduled only after its own
+  // wait): run beside it, and wait for it only at the end, for the kernel behind this one
+  bool beside;
 };
 constexpr int kShrinkWarps = 8, kShrinkStages = 2, kShrinkK = 64, kShrinkMaxCluster = 8;
 
@@ -93,6 +96,53 @@ __device__ __forceinline__ uint4 ld_shared_16(uint32_t addr) {
   return v;
 }
 
+// The last step of both kernels below: the blocks of a cluster add their sums [row][COLS] up in order and write V.
+template <int COLS>
+__device__ __forceinline__ void shrink_finish(const ShrinkArgs& args, const ShrinkProblem& pr, int chunk, const float* block_sums, const int* id_of,
+                                              int row0, int elems) {
+  const int rank = blockIdx.y, ranks = gridDim.y;
+  if (ranks > 1) {
+    cluster_arrive();
+    cluster_wait();
+  }
+  const int64_t ldv = (int64_t)args.terms * args.rp;
+  const uint32_t base = smem_u32(block_sums);
+  const int share = (elems + ranks - 1) / ranks, e_end = min(elems, (rank + 1) * share);
+  for (int e = rank * share + threadIdx.x; e < e_end; e += 32 * kShrinkWarps) {
+    const int lr = e / COLS, c = e % COLS, r = chunk * 64 + c;
+    const int a = id_of[lr];
+    if (a < 0) continue;
+    float v = 0.f;
+    if (ranks == 1) {
+      v = block_sums[e];
+    } else {
+      float part[kShrinkMaxCluster];
+#pragma unroll
+      for (int b = 0; b < kShrinkMaxCluster; ++b) part[b] = b < ranks ? ld_shared_cluster_f32(map_to_cta(base + 4u * (uint32_t)e, (uint32_t)b)) : 0.f;
+#pragma unroll
+      for (int b = 0; b < kShrinkMaxCluster; ++b) v += part[b];
+    }
+    v = r < args.R ? v : 0.f;
+    if (a >= args.n) v = NAN;
+    else if (r < args.R && args.scales) v *= args.scales[a];
+    __nv_bfloat16* dst = pr.V + (row0 + lr) * ldv + r;
+    const long long v_bytes = (long long)args.T * ldv * 2;
+    (void)v_bytes;
+    for (int t = 0; t < args.terms; ++t) {
+      const __nv_bfloat16 h = __float2bfloat16_rn(v);
+      if (GEMM_B200_IN_BOUNDS(dst + t * args.rp, pr.V, v_bytes, 2, 50)) dst[t * args.rp] = h;
+      const float back = __bfloat162float(h);
+      v = isinf(back) ? 0.f : v - back;   // an infinity is whole in its first summand
+    }
+  }
+  if (args.beside) pdl_wait();
+  __syncwarp();
+  if (ranks > 1) {   // no block leaves while another one reads its sums
+    cluster_arrive();
+    cluster_wait();
+  }
+}
+
 __device__ __forceinline__ int shrink_swizzle(int row) { return (row & 1) << 2 | (row >> 1 & 3); }
 
 template <int MT, int NT8>
@@ -109,7 +159,7 @@ lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
   const ShrinkProblem& pr = args.p[blockIdx.z / args.chunks];
   const int row0 = blockIdx.x * args.rows_per_block;
   const int row_end = min(args.T, row0 + args.rows_per_block);
-  pdl_wait();
+  if (!args.beside) pdl_wait();
   pdl_launch_dependents();
 
   TileIds<WORDS> ids;
@@ -244,44 +294,178 @@ lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
     }
   }
   __syncthreads();
-  if (ranks > 1) {
-    cluster_arrive();
-    cluster_wait();
+  shrink_finish<S::COLS>(args, pr, chunk, block_sums, id_of, row0, elems);
+}
+
+// The same for many rows: 16 * MT of them per block, with TMA.  Every warp takes each eighth step of 64 k and runs two rings of
+// its own, X tiles (all rows of the block) and A tiles (one adapter each); one lane asks for the tile after next once
+// the current one has been multiplied, so a step costs the warp its reads from shared memory and
+// its products.  (With the copies of the kernel above, addresses and predicates were half of the instructions: 8192 x
+// 8192, one adapter per 512 rows, 41 us; now REPLACE_ROWS.)  The adapters of a block share the X fragments, and a row
+// takes up the products of its own adapter only: by selection, so that nothing of another one reaches it.
+// Bound by the read of X.
+struct ShrinkMaps {
+  CUtensorMap x[2], a[2];   // x: box 64 k x ROWS rows; a: [adapters][R][K], box 64 k x COLS ranks
+};
+template <int MT, int NT8>
+struct ShrinkRowsShape {
+  static constexpr int ROWS = 16 * MT, COLS = 8 * NT8, LD = COLS + 8;
+  static constexpr int X_BYTES = ROWS * 128, A_BYTES = COLS * 128, WARP_BYTES = 2 * (X_BYTES + A_BYTES);
+  static constexpr int SUM_BYTES = (kShrinkWarps * ROWS * LD + ROWS * COLS) * 4;   // take the place of the rings
+  static constexpr int SMEM_BYTES = 1024 + kShrinkWarps * WARP_BYTES;
+  static_assert(SUM_BYTES <= kShrinkWarps * WARP_BYTES && SMEM_BYTES <= 231424, "shared memory budget");
+};
+
+template <int MT, int NT8>
+__global__ void __launch_bounds__(32 * kShrinkWarps, 1)
+lora_shrink_rows_kernel(const __grid_constant__ ShrinkArgs args, const __grid_constant__ ShrinkMaps maps) {
+  using S = ShrinkRowsShape<MT, NT8>;
+  constexpr int WORDS = (S::ROWS + 31) / 32;
+  extern __shared__ uint8_t shrink_rows_raw[];
+  uint8_t* smem = shrink_rows_raw + ((1024u - (smem_u32(shrink_rows_raw) & 1023u)) & 1023u);
+  __shared__ int id_of[S::ROWS], slot_id[S::ROWS], slot_count;
+  __shared__ __align__(8) uint64_t bars[kShrinkWarps * 4];
+  const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
+  const int rank = blockIdx.y, ranks = gridDim.y;
+  const int chunk = blockIdx.z % args.chunks, problem = blockIdx.z / args.chunks;
+  const ShrinkProblem& pr = args.p[problem];
+  const int row0 = blockIdx.x * S::ROWS, row_end = min(args.T, row0 + S::ROWS);
+  const uint32_t x_ring = smem_u32(smem) + warp * S::WARP_BYTES, a_ring = x_ring + 2 * S::X_BYTES;
+  const uint32_t x_bar = smem_u32(bars) + warp * 32, a_bar = x_bar + 16;
+  if (lane == 0) {
+    for (int i = 0; i < 4; ++i) mbar_init(x_bar + 8 * i, 1);
+    fence_mbar_init();
   }
-  const int64_t ldv = (int64_t)args.terms * args.rp;
-  const uint32_t base = smem_u32(block_sums);
-  const int share = (elems + ranks - 1) / ranks, e_end = min(elems, (rank + 1) * share);
-  for (int e = rank * share + threadIdx.x; e < e_end; e += 32 * kShrinkWarps) {
-    const int lr = e / S::COLS, c = e % S::COLS, r = chunk * 64 + c;
-    const int a = id_of[lr];
-    if (a < 0) continue;
-    float v = 0.f;
-    if (ranks == 1) {
-      v = block_sums[e];
-    } else {
-      float part[kShrinkMaxCluster];
+  if (!args.beside) pdl_wait();
+  pdl_launch_dependents();
+  if (warp == 0) {   // the block's rows and its distinct adapters, ascending
+    TileIds<WORDS> ids;
+    ids.load(args.ids, row0, row_end, lane);
 #pragma unroll
-      for (int b = 0; b < kShrinkMaxCluster; ++b) part[b] = b < ranks ? ld_shared_cluster_f32(map_to_cta(base + 4u * (uint32_t)e, (uint32_t)b)) : 0.f;
+    for (int w = 0; w < WORDS; ++w)
+      if (32 * w + lane < S::ROWS) id_of[32 * w + lane] = ids.id[w];
+    int count = 0;
+    for (int a = ids.next(); a >= 0 && a < args.n; a = ids.next(), ++count)
+      if (lane == 0) slot_id[count] = a;
+    if (lane == 0) slot_count = count;
+  }
+  __syncthreads();
+  const int slots = slot_count;
+  int id[MT][2];
 #pragma unroll
-      for (int b = 0; b < kShrinkMaxCluster; ++b) v += part[b];
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) id[mt][h] = id_of[mt * 16 + h * 8 + g];
+  const int steps = (pr.K + kShrinkK - 1) / kShrinkK, per = (steps + ranks - 1) / ranks;
+  const int step0 = min(steps, rank * per) + warp, step1 = min(steps, (rank + 1) * per);
+  const bool issuer = elect_one();
+
+  auto load_x = [&](int step, uint32_t buf) {
+    if (step < step1 && issuer) {
+      mbar_arrive_expect_tx(x_bar + 8 * buf, S::X_BYTES);
+      tma_load_3d(x_ring + buf * S::X_BYTES, &maps.x[problem], step * kShrinkK, row0, 0, x_bar + 8 * buf);
     }
-    v = r < args.R ? v : 0.f;
-    if (a < args.n && r < args.R && args.scales) v *= args.scales[a];
-    __nv_bfloat16* dst = pr.V + (row0 + lr) * ldv + r;
-    const long long v_bytes = (long long)args.T * ldv * 2;
-    (void)v_bytes;
-    for (int t = 0; t < args.terms; ++t) {
-      const __nv_bfloat16 h = __float2bfloat16_rn(v);
-      if (GEMM_B200_IN_BOUNDS(dst + t * args.rp, pr.V, v_bytes, 2, 50)) dst[t * args.rp] = h;
-      const float back = __bfloat162float(h);
-      v = isinf(back) ? 0.f : v - back;   // an infinity is whole in its first summand
+  };
+  int next_step = step0, next_slot = 0;   // the A tile to ask for next
+  auto load_a = [&](uint32_t buf) {
+    if (next_step < step1) {
+      if (issuer) {
+        mbar_arrive_expect_tx(a_bar + 8 * buf, S::A_BYTES);
+        tma_load_3d(a_ring + buf * S::A_BYTES, &maps.a[problem], next_step * kShrinkK, chunk * 64, slot_id[next_slot], a_bar + 8 * buf);
+      }
+      if (++next_slot == slots) { next_slot = 0; next_step += kShrinkWarps; }
+    }
+  };
+  float acc[MT][NT8][4] = {};
+  bool failed = false;
+  if (slots > 0) {
+    load_x(step0, 0);
+    load_a(0);
+    load_x(step0 + kShrinkWarps, 1);
+    load_a(1);
+  }
+  // tiles lie in 128-byte swizzled rows: unit u of row r at u ^ (r & 7); every row read here is g mod 8
+  const uint32_t unit[2] = {(uint32_t)(q ^ g) << 4, (uint32_t)((4 + q) ^ g) << 4};
+  uint32_t it = 0, item = 0;
+  for (int step = step0; step < step1 && slots > 0 && !failed; step += kShrinkWarps, ++it) {
+    const uint32_t xb = it & 1u, xs = x_ring + xb * S::X_BYTES + (uint32_t)g * 128u;
+    if (!mbar_wait_warp(x_bar + 8 * xb, (it >> 1) & 1u, kRoleMma, (int)xb)) { failed = true; break; }
+    uint4 x[MT][2][2];   // [16 rows][half of k][rows 0-7, 8-15]
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) x[mt][half][h] = ld_shared_16(xs + mt * 2048 + h * 1024 + unit[half]);
+    for (int slot = 0; slot < slots; ++slot, ++item) {
+      const uint32_t ab = item & 1u, as = a_ring + ab * S::A_BYTES + (uint32_t)g * 128u;
+      if (!mbar_wait_warp(a_bar + 8 * ab, (item >> 1) & 1u, kRoleMma, 2 + (int)ab)) { failed = true; break; }
+      uint4 w[2][NT8];
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int nt = 0; nt < NT8; ++nt) w[half][nt] = ld_shared_16(as + nt * 1024 + unit[half]);
+      const int a = slot_id[slot];
+#pragma unroll
+      for (int mt = 0; mt < MT; ++mt) {
+        // 64 k at a time in the tensor cores (which cut off low bits of a long running sum), added up in FP32
+        float t[NT8][4];
+#pragma unroll
+        for (int nt = 0; nt < NT8; ++nt)
+          mma_m16n8k16_bf16_zero(t[nt], x[mt][0][0].x, x[mt][0][1].x, x[mt][0][0].y, x[mt][0][1].y, w[0][nt].x, w[0][nt].y);
+#pragma unroll
+        for (int nt = 0; nt < NT8; ++nt)
+          mma_m16n8k16_bf16(t[nt], x[mt][0][0].z, x[mt][0][1].z, x[mt][0][0].w, x[mt][0][1].w, w[0][nt].z, w[0][nt].w);
+#pragma unroll
+        for (int nt = 0; nt < NT8; ++nt)
+          mma_m16n8k16_bf16(t[nt], x[mt][1][0].x, x[mt][1][1].x, x[mt][1][0].y, x[mt][1][1].y, w[1][nt].x, w[1][nt].y);
+#pragma unroll
+        for (int nt = 0; nt < NT8; ++nt)
+          mma_m16n8k16_bf16(t[nt], x[mt][1][0].z, x[mt][1][1].z, x[mt][1][0].w, x[mt][1][1].w, w[1][nt].z, w[1][nt].w);
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          if (id[mt][h] == a) {
+#pragma unroll
+            for (int nt = 0; nt < NT8; ++nt) {
+              acc[mt][nt][2 * h] += t[nt][2 * h];
+              acc[mt][nt][2 * h + 1] += t[nt][2 * h + 1];
+            }
+          }
+      }
+      // The products above were issued, so every fragment had arrived in its register: the tiles may be
+      // overwritten.  (Asked for right behind the reads, a tile could land before a read that was still queued.)
+      __syncwarp();
+      load_a(ab);
+      if (slot == 0) load_x(step + 2 * kShrinkWarps, xb);
     }
   }
-  __syncwarp();
-  if (ranks > 1) {   // no block leaves while another one reads its sums
-    cluster_arrive();
-    cluster_wait();
+  if (failed || aborted()) {   // copies in flight land before shared memory goes away
+    const unsigned long long t0 = globaltimer_ns();
+    while (globaltimer_ns() - t0 < 200000ull) __nanosleep(1000);
   }
+  __syncthreads();
+  float* warp_sums = reinterpret_cast<float*>(smem);                                   // [warp][row][LD]
+  float* block_sums = warp_sums + kShrinkWarps * S::ROWS * S::LD;                      // [row][COLS]
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float* dst = warp_sums + (warp * S::ROWS + mt * 16 + h * 8 + g) * S::LD + 2 * q;
+#pragma unroll
+      for (int nt = 0; nt < NT8; ++nt)
+        *reinterpret_cast<float2*>(dst + nt * 8) = make_float2(acc[mt][nt][2 * h], acc[mt][nt][2 * h + 1]);
+    }
+  __syncthreads();
+  const int elems = (row_end - row0) * S::COLS;
+  for (int e = threadIdx.x; e < elems; e += 32 * kShrinkWarps) {
+    const int lr = e / S::COLS, c = e % S::COLS;
+    float sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kShrinkWarps; ++w) sum += warp_sums[(w * S::ROWS + lr) * S::LD + c];
+    block_sums[e] = sum;
+  }
+  __syncthreads();
+  shrink_finish<S::COLS>(args, pr, chunk, block_sums, id_of, row0, elems);
 }
 
 // ---------------------------------------------------------------------------------------
