@@ -37,11 +37,11 @@ SIGNATURES = {
     "gemm_b200_gemm_bf16_num_configs": (i32, []),
     "gemm_b200_gemm_bf16_config_name": (C.c_char_p, [i32]),
     "gemm_b200_gemm_bf16_xent": (i32, [vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, vp, sz, vp]),
-    "gemm_b200_gemm_bf16_xent_scratch_bytes": (sz, [i64, i64, i64]),
+    "gemm_b200_gemm_bf16_xent_scratch_bytes": (sz, [i64, i64]),
     "gemm_b200_gemm_bf16_xent_grad": (i32, [vp, vp, vp, vp, vp, i64, vp, i64, vp, vp, i64, i64, i64, i64, i64, i64, i64, vp, sz, vp]),
     "gemm_b200_gemm_bf16_xent_grad_scratch_bytes": (sz, [i64, i64, i64]),
     "gemm_b200_gemm_bf16_lora": (i32, [vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, i32, i32, vp, sz, vp]),
-    "gemm_b200_gemm_bf16_lora_scratch_bytes": (sz, [i64, i64, i64, i64, i32]),
+    "gemm_b200_gemm_bf16_lora_scratch_bytes": (sz, [i64, i64, i64, i64, i64, i32]),
     "gemm_b200_gemm_bf16_lora_grad": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, i64, i32, vp, sz, vp]),
     "gemm_b200_gemm_bf16_lora_grad_scratch_bytes": (sz, [i64, i64, i64, i64, i64, i32]),
     "gemm_b200_quantize_mxfp8": (i32, [vp, i64, i64, i64, i32, vp, vp, vp]),

@@ -87,24 +87,31 @@ static bool bf16_pairs_dynamic(int64_t M, int64_t N, int64_t K, int sms) {
   return units > sms / 2 && K >= 6144;
 }
 
+// A product of one row tile, 128 x 256 tiles of single CTAs, the box of A by the number of rows.
+template <int A_ROWS>
+using Bf16_row_tile = Bf16Cfg<1, A_ROWS == 32 ? 5 : 4, 1, false, 1, 2, kBlockN, false, 0, A_ROWS>;
+template <bool B_MN, bool OUT_F32, class Fuse>
+static int launch_row_tile(const Bf16Args& a, const Fuse& fuse) {
+  if (a.M <= 32) return launch_bf16_fused<Bf16_row_tile<32>, B_MN, OUT_F32, false, Fuse>(a, fuse);
+  if (a.M <= 64) return launch_bf16_fused<Bf16_row_tile<64>, B_MN, OUT_F32, false, Fuse>(a, fuse);
+  return launch_bf16_fused<Bf16_1cta_tma, B_MN, OUT_F32, false, Fuse>(a, fuse);
+}
+
 // =========================================================================================
 // Softmax cross entropy
 // =========================================================================================
-// One row tile streams W once: 128-column tiles, so that the last round of tiles over the SMs is fuller.
-using Xent_1cta = Bf16Cfg<1, 7, 0, false, 1, 0, 128, false, 8>;
+// One row tile streams W once, with a box of X that fits the rows (A_ROWS in gemm_bf16.cuh).
+template <int A_ROWS>
+using Xent_1cta = Bf16Cfg<1, A_ROWS == 128 ? 4 : 5, 0, false, 1, 0, kBlockN, false, 8, A_ROWS>;
 using Xent_2cta = Bf16Cfg<2, 7, 0, true, 1, 0, kBlockN, false, 8>;
 using Xent_2cta_dyn = Bf16Cfg<2, 7, 0, true, 1, 0, kBlockN, true, 8>;
 
 struct XentScratch {
   float2* part;
   float* label_logit;
-  __nv_bfloat16* xp;   // X padded to kMinMapRows rows
-  int64_t ldp;
   size_t bytes;
-  XentScratch(void* base, int64_t T, int64_t V, int64_t D) {
+  XentScratch(void* base, int64_t T, int64_t V) {
     Carver c{static_cast<char*>(base)};
-    ldp = ceil_div64(D, 8) * 8;
-    xp = c.take<__nv_bfloat16>(T < kMinMapRows ? kMinMapRows * ldp : 0);
     part = c.take<float2>(ceil_div64(V, kXentCols) * T);
     label_logit = c.take<float>(T);
     bytes = c.used;
@@ -146,10 +153,9 @@ struct XentGradScratch {
   XentGradScratch(void* base, int64_t T, int64_t D, const XentGradPlan& p) {
     Carver c{static_cast<char*>(base)};
     ldd = ceil_div64(p.piece, 8) * 8;
-    const int64_t map_rows = T < kMinMapRows ? kMinMapRows : T;
     rows = c.take<XentRow>(T);
-    xw = c.take<__nv_bfloat16>(map_rows * D);
-    d = c.take<__nv_bfloat16>(map_rows * ldd);
+    xw = c.take<__nv_bfloat16>(T * D);
+    d = c.take<__nv_bfloat16>(T * ldd);
     dx = c.take<float>(p.dx_acc ? (int64_t)p.dx_splits * T * D : 0);
     dw = c.take<float>(p.dw_splits > 1 ? (int64_t)p.dw_splits * p.piece * D : 0);
     bytes = c.used;
@@ -159,7 +165,7 @@ struct XentGradScratch {
 // FP32 tiles of A @ B into the slices at a.C: stored (first) or added to what is there.
 template <class Fuse>
 static int launch_bf16_slices(const Bf16Args& a, const Fuse& fuse, int sms) {
-  if (a.M <= kBlockM) return launch_bf16_fused<Bf16_1cta_tma, true, true, false, Fuse>(a, fuse);
+  if (a.M <= kBlockM) return launch_row_tile<true, true>(a, fuse);
   if (a.k_splits == 1 && bf16_pairs_dynamic(a.M, a.N, a.K, sms))
     return launch_bf16_fused<Bf16_2cta_tma_m_dyn, true, true, false, Fuse>(a, fuse);
   return launch_bf16_fused<Bf16_2cta_tma_m, true, true, false, Fuse>(a, fuse);
@@ -173,23 +179,17 @@ static int xent_entry(const void* X, const void* W, const int64_t* labels, float
   if (!aligned16(X) || !aligned16(W) || ldx % 8 != 0 || ldw % 8 != 0)
     return fail(GEMM_B200_ERR_ALIGNMENT, "gemm_bf16_xent: X and W must be 16-byte aligned, ldx and ldw multiples of 8 (ldx=%lld ldw=%lld)",
                 (long long)ldx, (long long)ldw);
-  const XentScratch ws(scratch, T, V, D);
+  const XentScratch ws(scratch, T, V);
   if (int rc = check_scratch("gemm_bf16_xent", scratch, scratch_bytes, ws.bytes)) return rc;
   DeviceInfo di;
   if (int rc = check_blackwell("gemm_bf16_xent", &di)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  Bf16Args a{X, W, nullptr, T, V, D, ldx, ldw, V, st};
+  const Bf16Args a{X, W, nullptr, T, V, D, ldx, ldw, V, st};
   const XentStatsFuse fuse{ws.part, ws.label_logit, labels};
   int rc;
-  if (T < kMinMapRows) {
-    if ((rc = launch_plain(xent_pad_kernel, dim3((unsigned)kMinMapRows), 128, 0, 1, st, static_cast<const __nv_bfloat16*>(X), ldx, ws.xp, ws.ldp,
-                           (int)T, (int)D)))
-      return rc;
-    a.A = ws.xp;
-    a.lda = ws.ldp;
-    a.a_rows = kMinMapRows;
-  }
-  if (T <= kBlockM) rc = launch_bf16_fused<Xent_1cta, false, true>(a, fuse);
+  if (T <= 32) rc = launch_bf16_fused<Xent_1cta<32>, false, true>(a, fuse);
+  else if (T <= 64) rc = launch_bf16_fused<Xent_1cta<64>, false, true>(a, fuse);
+  else if (T <= kBlockM) rc = launch_bf16_fused<Xent_1cta<128>, false, true>(a, fuse);
   else if (bf16_pairs_dynamic(T, V, D, di.sms)) rc = launch_bf16_fused<Xent_2cta_dyn, false, true>(a, fuse);
   else rc = launch_bf16_fused<Xent_2cta, false, true>(a, fuse);
   if (rc) return rc;
@@ -231,31 +231,26 @@ static int xent_grad_entry(const void* X, const void* W, const int64_t* labels, 
   if (log_enabled())
     fprintf(stderr, "[gemm_b200] gemm_bf16_xent_grad T=%lld V=%lld D=%lld -> %lld pieces of %lld, K ranges %d (dX) %d (dW)\n", (long long)T,
             (long long)V, (long long)D, (long long)plan.pieces, (long long)plan.piece, plan.dx_splits, plan.dw_splits);
-  const int64_t a_rows = T < kMinMapRows ? kMinMapRows : 0;
-  if (int rc = launch_plain(xent_prepare_kernel, dim3((unsigned)(a_rows ? a_rows : T)), 128, 0, 1, st, labels, lse, grad_loss, grad_loss_stride,
-                            grad_lse, grad_lse_stride, static_cast<const __nv_bfloat16*>(X), ldx, ws.rows, ws.xw, (int)T, (int)D, (int)V))
+  if (int rc = launch_plain(xent_prepare_kernel, dim3((unsigned)T), 128, 0, 1, st, labels, lse, grad_loss, grad_loss_stride, grad_lse,
+                            grad_lse_stride, static_cast<const __nv_bfloat16*>(X), ldx, ws.rows, ws.xw, (int)D, (int)V))
     return rc;
   int dx_slices = 1;
   for (int64_t v0 = 0; v0 < V; v0 += plan.piece) {
     const int64_t n = V - v0 < plan.piece ? V - v0 : plan.piece;
     const char* Wp = static_cast<const char*>(W) + v0 * ldw * 2;
     // d of the piece
-    Bf16Args z{X, Wp, ws.d, T, n, D, ldx, ldw, ws.ldd, st};
-    if (a_rows) {   // rows without weight are zeros there: their logits count for nothing
-      z.A = ws.xw;
-      z.lda = D;
-      z.a_rows = a_rows;
-    }
+    const Bf16Args z{X, Wp, ws.d, T, n, D, ldx, ldw, ws.ldd, st};
     const XentGradFuse fuse{ws.rows, (int)v0};
     int rc;
-    if (T <= kBlockM) rc = launch_bf16_fused<Bf16_1cta_tma, false, false>(z, fuse);
+    if (T <= kBlockM) rc = launch_row_tile<false, false>(z, fuse);
     else if (bf16_pairs_dynamic(T, n, D, di.sms)) rc = launch_bf16_fused<Bf16_2cta_tma_m_dyn, false, false>(z, fuse);
     else rc = launch_bf16_fused<Bf16_2cta_tma_m, false, false>(z, fuse);
     if (rc) return rc;
     // dX (+)= d W
     Bf16Args gx{ws.d, Wp, dX, T, D, n, ws.ldd, ldw, lddx, st};
-    gx.a_rows = a_rows;   // rows of d above T hold anything and reach only rows of the product above T
-    if (!plan.dx_acc) {
+    if (!plan.dx_acc && T <= kBlockM) {
+      rc = launch_row_tile<true, false>(gx, NoFuse());
+    } else if (!plan.dx_acc) {
       rc = kBf16Configs[pick_bf16_config(T, D, n, di.sms)].launch[GEMM_B200_B_ROW_MAJOR_KN][GEMM_B200_OUT_BF16](gx);
     } else {
       gx.C = ws.dx;
@@ -313,10 +308,11 @@ static int lora_sizes(const char* who, int64_t T, int64_t N, int64_t D, int64_t 
   return GEMM_B200_OK;
 }
 
-// K over the blocks of a cluster until most SMs have one, as long as every block keeps a step of its eight warps.
-static int shrink_cluster(int64_t blocks, int64_t max_k, const DeviceInfo& di) {
+// K over the blocks of a cluster: the largest that keeps the grid within `places`, as long as every block keeps a step
+// of its eight warps.
+static int shrink_cluster(int64_t blocks, int64_t max_k, int64_t places) {
   int ks = 1;
-  while (ks < kShrinkMaxCluster && 5 * blocks * ks < 4 * (int64_t)di.sms && max_k / (kShrinkK * kShrinkWarps) >= 2 * ks) ks *= 2;
+  while (ks < kShrinkMaxCluster && blocks * 2 * ks <= places && max_k / (kShrinkK * kShrinkWarps) >= 2 * ks) ks *= 2;
   return ks;
 }
 
@@ -325,10 +321,11 @@ static int launch_shrink_few(ShrinkArgs args, int problems, int64_t max_k, const
   using S = ShrinkShape<1, NT8>;
   auto kern = lora_shrink_kernel<1, NT8>;
   if (int rc = allow_smem(kern, S::SMEM_BYTES, di)) return rc;
-  // a block per row, so that every adapter streams on its own; from 65 rows on 16 share a block
-  args.rows_per_block = args.T <= 64 ? 1 : S::ROWS;
+  // a block per row, so that every adapter streams on its own; from 65 rows on four share a block (97 rows of 32
+  // requests, rank 113: 32 us with sixteen, whose adapters a warp takes one after another)
+  args.rows_per_block = args.T <= 64 ? 1 : 4;
   const int64_t blocks = ceil_div64(args.T, args.rows_per_block), z = problems * args.chunks;
-  const int ks = shrink_cluster(blocks * z, max_k, di);
+  const int ks = shrink_cluster(blocks * z, max_k, 4 * (int64_t)di.sms);   // rows without an adapter leave at once
   return launch_plain(kern, dim3((unsigned)blocks, (unsigned)ks, (unsigned)z), 32 * kShrinkWarps, S::SMEM_BYTES, ks, st, args);
 }
 
@@ -349,7 +346,7 @@ static int launch_shrink_rows(ShrinkArgs args, int problems, int64_t max_k, cons
       return rc;
   }
   const int64_t blocks = ceil_div64(args.T, S::ROWS), z = problems * args.chunks;
-  const int ks = shrink_cluster(blocks * z, max_k, di);
+  const int ks = shrink_cluster(blocks * z, max_k, di.sms);                // a block has its SM to itself
   return launch_plain(kern, dim3((unsigned)blocks, (unsigned)ks, (unsigned)z), 32 * kShrinkWarps, S::SMEM_BYTES, ks, st, args, maps);
 }
 
@@ -377,14 +374,52 @@ struct LoraScratch {
   }
 };
 
-// the tile shapes of bf16 results, and those of FP32 ones (accumulators drained every 512 of K)
-using Lora_1cta_f32 = Bf16Cfg<1, 6, 1, false, 1, 2, 128, false, 8>;
+// the tile shapes of FP32 results: accumulators drained every 512 of K
+template <int A_ROWS>
+using Lora_row_tile_f32 = Bf16Cfg<1, A_ROWS == 32 ? 5 : 4, 1, false, 1, 1, kBlockN, false, 8, A_ROWS>;
 using Lora_2cta_f32 = Bf16Cfg<2, 6, 1, true, 1, 1, kBlockN, false, 8>;
 using Lora_2cta_f32_dyn = Bf16Cfg<2, 6, 1, true, 1, 1, kBlockN, true, 8>;
 
-template <class Cfg, bool F32>
-static int launch_lora(const Bf16Args& a, const LoraFuse& fuse, int b_layout) {
-  return b_layout == GEMM_B200_B_ROW_MAJOR_KN ? launch_bf16_fused<Cfg, true, F32>(a, fuse) : launch_bf16_fused<Cfg, false, F32>(a, fuse);
+// f32: an FP32 result; otherwise bf16, or the FP32 slices of one that is split over K
+template <bool B_MN>
+static int launch_lora(const Bf16Args& a, const LoraFuse& fuse, bool f32, int sms) {
+  if (a.M <= kBlockM) {
+    if (!f32) return a.k_splits > 1 ? launch_row_tile<B_MN, true>(a, fuse) : launch_row_tile<B_MN, false>(a, fuse);
+    if (a.M <= 32) return launch_bf16_fused<Lora_row_tile_f32<32>, B_MN, true>(a, fuse);
+    if (a.M <= 64) return launch_bf16_fused<Lora_row_tile_f32<64>, B_MN, true>(a, fuse);
+    return launch_bf16_fused<Lora_row_tile_f32<128>, B_MN, true>(a, fuse);
+  }
+  if (a.k_splits > 1) return f32 ? launch_bf16_fused<Lora_2cta_f32, B_MN, true>(a, fuse) : launch_bf16_fused<Bf16_2cta_tma_m, B_MN, true>(a, fuse);
+  if (bf16_pairs_dynamic(a.M, a.N, a.K, sms))
+    return f32 ? launch_bf16_fused<Lora_2cta_f32_dyn, B_MN, true>(a, fuse) : launch_bf16_fused<Bf16_2cta_tma_m_dyn, B_MN, false>(a, fuse);
+  return f32 ? launch_bf16_fused<Lora_2cta_f32, B_MN, true>(a, fuse) : launch_bf16_fused<Bf16_2cta_tma_m, B_MN, false>(a, fuse);
+}
+
+// K ranges of the projection: the estimate of bf16_auto_splits with the adapters' K blocks, which the ranges share, beside
+// those of D.  How many adapters a row tile has is known on the device only: a decoding batch (one row tile) is taken
+// to have one per row, longer ones (prompts, whose rows of one request lie together) half of that.
+static int lora_splits(int64_t T, int64_t N, int64_t D, int64_t R, int64_t n, int terms, int sms) {
+  const bool pair = bf16_splitk_pairs(T);
+  const int64_t rows = pair ? 2 * kBlockM : kBlockM, rp = lora_rp(R);
+  const int64_t tiles = ceil_div64(T, rows) * ceil_div64(N, kBlockN), slots = pair ? sms / 2 : sms;
+  const int64_t num_kb = ceil_div64(D, kBlockK);
+  int64_t ads = T < rows ? T : rows;
+  if (n < ads) ads = n;
+  if (pair) ads = (ads + 1) / 2;
+  const int64_t ad_kb = rp <= 64 ? ceil_div64(ads, 64 / rp) * ceil_div64(terms * rp, 64) : ads * terms * (rp / 64);
+  if (3 * tiles >= 2 * slots || num_kb + ad_kb < 32) return 1;
+  const double t_kb = pair ? 0.30 : 0.39, slice_us = (double)T * (double)N * 8.0 / 7.8e6;
+  double best_cost = (double)(num_kb + ad_kb) * t_kb;   // less than one round: see above
+  int best = 1;
+  for (int s = 2; s <= 32; ++s) {
+    const int64_t kb_per = ceil_div64(num_kb, s), per = kb_per + ceil_div64(ad_kb, s);
+    if (kb_per < 2 || per < 8) break;                                    // at least 512 of K per range
+    if ((double)s * (double)T * (double)N * 4.0 > 268435456.0) break;   // scratch of at most 256 MiB
+    if (ceil_div64(num_kb, kb_per) != s) continue;                      // no empty range
+    const double cost = (double)ceil_div64(tiles * s, slots) * (double)per * t_kb + s * slice_us + 6.0;
+    if (cost < best_cost) { best_cost = cost; best = s; }
+  }
+  return best;
 }
 
 static int lora_entry(const void* X, const void* W, const void* A, const void* B, const int32_t* ids, const float* scales, void* Y,
@@ -403,7 +438,7 @@ static int lora_entry(const void* X, const void* W, const void* A, const void* B
     return fail(GEMM_B200_ERR_ALIGNMENT, "gemm_bf16_lora: X, W, A, B and Y must be 16-byte aligned, ldw a multiple of 8, ldy*sizeof(Y) of 16 bytes");
   DeviceInfo di;
   if (int rc = check_blackwell("gemm_bf16_lora", &di)) return rc;
-  const int splits = bf16_auto_splits(T, N, D, di.sms), terms = lora_terms(out_dtype), rp = lora_rp(R);
+  const int terms = lora_terms(out_dtype), rp = lora_rp(R), splits = lora_splits(T, N, D, R, n, terms, di.sms);
   const LoraScratch ws(scratch, T, N, R, terms, splits);
   if (int rc = check_scratch("gemm_bf16_lora", scratch, scratch_bytes, ws.bytes)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -422,7 +457,7 @@ static int lora_entry(const void* X, const void* W, const void* A, const void* B
 
   LoraFuse fuse;
   if (int rc = make_map_3d(&fuse.tmV, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ws.V, T, (int64_t)terms * rp, (int64_t)terms * rp, 1,
-                           T * terms * rp, kBlockK, kBlockM, CU_TENSOR_MAP_SWIZZLE_128B))
+                           T * terms * rp, kBlockK, T <= 32 ? 32 : T <= 64 ? 64 : kBlockM, CU_TENSOR_MAP_SWIZZLE_128B))   // the box of X's tiles
     return rc;
   if (int rc = make_map_3d(&fuse.tmAd, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, B, R, N, ldb, n, stride_b, 64, rp < 64 ? rp : 64,
                            CU_TENSOR_MAP_SWIZZLE_128B))
@@ -436,21 +471,10 @@ static int lora_entry(const void* X, const void* W, const void* A, const void* B
     a.C = ws.slices;
     a.ldc = N;
     a.k_splits = splits;
-    int rc;
-    if (f32) rc = bf16_splitk_pairs(T) ? launch_lora<Lora_2cta_f32, true>(a, fuse, w_layout) : launch_lora<Lora_1cta_f32, true>(a, fuse, w_layout);
-    else rc = bf16_splitk_pairs(T) ? launch_lora<Bf16_2cta_tma_m, true>(a, fuse, w_layout) : launch_lora<Bf16_1cta_tma, true>(a, fuse, w_layout);
-    if (rc) return rc;
-    const int64_t num_kb = ceil_div64(D, kBlockK);
-    return launch_splitk_reduce(ws.slices, T, N, (int)ceil_div64(num_kb, ceil_div64(num_kb, splits)), Y, ldy, out_dtype, st);
   }
-  const bool dynamic = bf16_pairs_dynamic(T, N, D, di.sms);
-  if (f32)
-    return T <= kBlockM ? launch_lora<Lora_1cta_f32, true>(a, fuse, w_layout)
-           : dynamic    ? launch_lora<Lora_2cta_f32_dyn, true>(a, fuse, w_layout)
-                        : launch_lora<Lora_2cta_f32, true>(a, fuse, w_layout);
-  return T <= kBlockM ? launch_lora<Bf16_1cta_tma, false>(a, fuse, w_layout)
-         : dynamic    ? launch_lora<Bf16_2cta_tma_m_dyn, false>(a, fuse, w_layout)
-                      : launch_lora<Bf16_2cta_tma_m, false>(a, fuse, w_layout);
+  const int rc = w_layout == GEMM_B200_B_ROW_MAJOR_KN ? launch_lora<true>(a, fuse, f32, di.sms) : launch_lora<false>(a, fuse, f32, di.sms);
+  if (rc || splits == 1) return rc;
+  return launch_splitk_reduce(ws.slices, T, N, splits, Y, ldy, out_dtype, st);
 }
 
 static int lora_grad_per_sm(int rp, int terms) {
@@ -460,25 +484,22 @@ static int lora_grad_per_sm(int rp, int terms) {
 }
 
 struct LoraGradPlan {
-  int64_t chunks_d, chunks_n, block_tokens, blocks;
+  int64_t chunks_d, chunks_n, blocks;
   LoraGradPlan(int64_t T, int64_t N, int64_t D, int64_t R, int terms, int sms) {
     chunks_d = ceil_div64(D, kGradCols);
     chunks_n = ceil_div64(N, kGradCols);
     // Blocks of tokens so that the grid fills one, two or three rounds of the resident thread blocks best (672 thread
-    // blocks on 444 places: a third of the second round idle), but not below 64 tokens.
-    const int64_t chunks = chunks_d + chunks_n, slots = (int64_t)sms * lora_grad_per_sm(lora_rp(R), terms), most = ceil_div64(T, 64);
-    int64_t want = 1;
+    // blocks on 444 places: a third of the second round idle), but not below four tokens.
+    const int64_t chunks = chunks_d + chunks_n, slots = (int64_t)sms * lora_grad_per_sm(lora_rp(R), terms), most = ceil_div64(T > 0 ? T : 1, 4);
+    blocks = 1;
     double best = 0;
     for (int rounds = 1; rounds <= 3; ++rounds) {
       int64_t b = rounds * slots / chunks;
       if (b < 1) b = 1;
       if (b > most) b = most;
       const double fill = (double)(b * chunks) / (double)(ceil_div64(b * chunks, slots) * slots);
-      if (fill > best + 0.03) { best = fill; want = b; }
+      if (fill > best + 0.03) { best = fill; blocks = b; }
     }
-    if (want < 1) want = 1;
-    block_tokens = ceil_div64(ceil_div64(T > 0 ? T : 1, want), kGradTokens) * kGradTokens;
-    blocks = ceil_div64(T > 0 ? T : 1, block_tokens);
   }
 };
 struct LoraGradScratch {
@@ -507,9 +528,10 @@ static int launch_lora_grad(const GradArgs& ga, const LoraGradPlan& plan, const 
   if (int rc = allow_smem(kern, smem, di)) return rc;
   if (int rc = launch_plain(kern, dim3((unsigned)(plan.chunks_d + plan.chunks_n), (unsigned)plan.blocks), kGradThreads, smem, 1, st, ga))
     return rc;
-  const int64_t most = (int64_t)ga.R * (ga.p[0].cols > ga.p[1].cols ? ga.p[0].cols : ga.p[1].cols);
-  int64_t bx = ceil_div64(most, 1024);
-  if (bx > 256) bx = 256;
+  // about eight blocks per SM over the adapters and both operands
+  const int64_t most = ceil_div64((int64_t)ga.R * (ga.p[0].cols > ga.p[1].cols ? ga.p[0].cols : ga.p[1].cols), 1024);
+  int64_t bx = ceil_div64(8 * (int64_t)di.sms, 2 * (int64_t)ga.n);
+  if (bx > most) bx = most;
   return launch_plain(lora_join_kernel<F32>, dim3((unsigned)bx, (unsigned)ga.n, 2), 256, 0, 1, st, ga);
 }
 
@@ -558,7 +580,7 @@ static int lora_grad_entry(const void* X, const void* dY, const void* A, const v
   ga.start = ws.start;
   ga.n = (int)n;
   ga.R = (int)R;
-  ga.block_tokens = (int)plan.block_tokens;
+  ga.blocks = (int)plan.blocks;
   if (terms == 1)
     return rp == 16 ? launch_lora_grad<1, 1>(ga, plan, di, st) : rp == 32 ? launch_lora_grad<2, 1>(ga, plan, di, st)
          : rp == 64 ? launch_lora_grad<4, 1>(ga, plan, di, st) : launch_lora_grad<8, 1>(ga, plan, di, st);
@@ -574,9 +596,9 @@ static int current_sms() {
 }  // namespace tc
 }  // namespace gemm_b200
 
-extern "C" size_t gemm_b200_gemm_bf16_xent_scratch_bytes(int64_t T, int64_t V, int64_t D) {
-  if (T <= 0 || V <= 0 || D <= 0) return 0;
-  return gemm_b200::tc::XentScratch(nullptr, T, V, D).bytes;
+extern "C" size_t gemm_b200_gemm_bf16_xent_scratch_bytes(int64_t T, int64_t V) {
+  if (T <= 0 || V <= 0) return 0;
+  return gemm_b200::tc::XentScratch(nullptr, T, V).bytes;
 }
 extern "C" int gemm_b200_gemm_bf16_xent(const void* X, const void* W, const int64_t* labels, float* loss, float* lse, int64_t T, int64_t V,
                                         int64_t D, int64_t ldx, int64_t ldw, void* scratch, size_t scratch_bytes, void* stream) {
@@ -595,11 +617,12 @@ extern "C" int gemm_b200_gemm_bf16_xent_grad(const void* X, const void* W, const
   return gemm_b200::tc::xent_grad_entry(X, W, labels, lse, grad_loss, grad_loss_stride, grad_lse, grad_lse_stride, dX, dW, T, V, D, ldx, ldw,
                                         lddx, lddw, scratch, scratch_bytes, stream);
 }
-extern "C" size_t gemm_b200_gemm_bf16_lora_scratch_bytes(int64_t T, int64_t N, int64_t D, int64_t R, int out_dtype) {
+extern "C" size_t gemm_b200_gemm_bf16_lora_scratch_bytes(int64_t T, int64_t N, int64_t D, int64_t R, int64_t adapters, int out_dtype) {
   using namespace gemm_b200::tc;
   const int sms = current_sms();
-  if (T <= 0 || N <= 0 || D <= 0 || R <= 0 || R > kLoraMaxRank || sms <= 0) return 0;
-  return LoraScratch(nullptr, T, N, R, lora_terms(out_dtype), bf16_auto_splits(T, N, D, sms)).bytes;
+  if (T <= 0 || N <= 0 || D <= 0 || R <= 0 || R > kLoraMaxRank || adapters <= 0 || sms <= 0) return 0;
+  const int terms = lora_terms(out_dtype);
+  return LoraScratch(nullptr, T, N, R, terms, lora_splits(T, N, D, R, adapters, terms, sms)).bytes;
 }
 extern "C" int gemm_b200_gemm_bf16_lora(const void* X, const void* W, const void* A, const void* B, const int32_t* ids, const float* scales,
                                         void* Y, int64_t T, int64_t N, int64_t D, int64_t R, int64_t adapters, int64_t ldx, int64_t ldw,

@@ -120,8 +120,12 @@ struct SchedRing {
 //     are FP32 for their precision are drained every ACC_KB blocks and added up in registers: 128 columns per epilogue
 //     warp, 5e-7 with 8 blocks (K = 512).  The drains use the two accumulator buffers in turn, as tiles do, and hide
 //     under the next blocks' products.
+// A_ROWS: rows of A a stage loads (the TMA box).  Fewer than 128 (M <= A_ROWS): the MMA still reads 128 rows of shared
+//     memory, whose upper ones hold another stage's bytes or stale ones; they reach only accumulator rows >= M, which are
+//     never stored.  Rows outside the matrix are not free to the copy engine: one row of A against 131072 x 4096, 187 us
+//     with 128-row boxes, 164 with 32-row ones; against 100000 x 2816, 107 and 86.
 template <int CG_, int STAGES_, int EPI_, bool COMMIT_MASK_, int NT_ = 1, int EPI_BUFS_ = (NT_ == 1 ? 2 : 1),
-          int BN_ = kBlockN, bool DYN_ = false, int ACC_KB_ = 0>
+          int BN_ = kBlockN, bool DYN_ = false, int ACC_KB_ = 0, int A_ROWS_ = kBlockM>
 struct Bf16Cfg {
   static constexpr int CG = CG_, STAGES = STAGES_, EPI = EPI_, NT = NT_, BN = BN_;
   static constexpr bool COMMIT_MASK = COMMIT_MASK_, DYN = DYN_;
@@ -132,17 +136,20 @@ struct Bf16Cfg {
   static constexpr int EPI_BUFS = EPI_BUFS_;                       // staging buffers per epilogue warp
   static constexpr int TILE_N = BN * NT;                       // columns of C per work unit
   static constexpr int BN_CTA = BN / CG;                       // columns of B each CTA loads per column tile
-  static constexpr int A_BYTES = kBlockM * kBlockK * 2;             // 16 KB
+  static constexpr int A_ROWS = A_ROWS_;
+  static constexpr int A_BYTES = A_ROWS * kBlockK * 2;              // 16 KB for 128 rows
+  static constexpr int A_TAIL = (kBlockM - A_ROWS) * kBlockK * 2;   // what the last stage's MMAs read beyond it
   static constexpr int B_BYTES = BN_CTA * kBlockK * 2;              // 32 KB / 16 KB, per column tile
   static constexpr int STAGE_BYTES = A_BYTES + NT * B_BYTES;
   static constexpr int EPI_WARP_BUF = 32 * 128;                     // 32 rows x 128 bytes
   static constexpr int EPI_BYTES = EPI_WARPS * EPI_BUFS * EPI_WARP_BUF;
   static constexpr int BAR_BYTES = (2 * STAGES + 4) * 8 + 16 + (DYN ? kSchedBytes : 0);
-  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + EPI_BYTES + BAR_BYTES;
+  static constexpr int SMEM_BYTES = 1024 + STAGES * STAGE_BYTES + A_TAIL + EPI_BYTES + BAR_BYTES;
   static_assert(STAGES + 5 <= kSchedSlots, "the unit ring must outlast the producer's lead over the epilogue");
   static_assert(NT == 1 || NT == 2, "column tiles per unit");
   static_assert(BN == 256 || (BN == 128 && NT == 1), "tile width");
   static_assert(SMEM_BYTES <= 232448, "shared memory budget");
+  static_assert(A_ROWS == kBlockM || (CG == 1 && A_ROWS % 8 == 0), "narrow A is for one row tile of a single CTA");
   static_assert(ACC_KB == 0 || NT == 1, "drained accumulators need two buffers");
 };
 
@@ -288,8 +295,8 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t sA0 = smem_base;
-  const uint32_t sB0 = smem_base + STAGES * Cfg::A_BYTES;     // [stage][column tile][B_BYTES]
-  const uint32_t sEpi0 = smem_base + STAGES * Cfg::STAGE_BYTES;
+  const uint32_t sB0 = smem_base + STAGES * Cfg::A_BYTES + Cfg::A_TAIL;     // [stage][column tile][B_BYTES]
+  const uint32_t sEpi0 = smem_base + STAGES * Cfg::STAGE_BYTES + Cfg::A_TAIL;
   const uint32_t bar0 = sEpi0 + Cfg::EPI_BYTES;
   auto full_bar = [&](int s) { return bar0 + 8u * s; };
   auto empty_bar = [&](int s) { return bar0 + 8u * (STAGES + s); };

@@ -298,19 +298,20 @@ lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
 }
 
 // The same for many rows: 16 * MT of them per block, with TMA.  Every warp takes each eighth step of 64 k and runs two rings of
-// its own, X tiles (all rows of the block) and A tiles (one adapter each); one lane asks for the tile after next once
-// the current one has been multiplied, so a step costs the warp its reads from shared memory and
+// its own, X tiles (all rows of the block) and A tiles (one adapter each); one lane asks for another tile once
+// the oldest one has been multiplied, so a step costs the warp its reads from shared memory and
 // its products.  (With the copies of the kernel above, addresses and predicates were half of the instructions: 8192 x
-// 8192, one adapter per 512 rows, 41 us; now REPLACE_ROWS.)  The adapters of a block share the X fragments, and a row
-// takes up the products of its own adapter only: by selection, so that nothing of another one reaches it.
-// Bound by the read of X.
+// 8192, one adapter per 512 rows, 41 us; now REPLACE_ROWS.)  The adapters of a block share the X tile, each multiplies the
+// groups of 16 rows that have it, and a row takes up the products of its own adapter only: by selection, so that
+// nothing of another one reaches it.  Bound by the read of X where the rows of a request lie together.
 struct ShrinkMaps {
   CUtensorMap x[2], a[2];   // x: box 64 k x ROWS rows; a: [adapters][R][K], box 64 k x COLS ranks
 };
 template <int MT, int NT8>
 struct ShrinkRowsShape {
   static constexpr int ROWS = 16 * MT, COLS = 8 * NT8, LD = COLS + 8;
-  static constexpr int X_BYTES = ROWS * 128, A_BYTES = COLS * 128, WARP_BYTES = 2 * (X_BYTES + A_BYTES);
+  static constexpr int A_STAGES = COLS == 16 ? 6 : COLS == 32 ? 3 : 2;      // as many as fit
+  static constexpr int X_BYTES = ROWS * 128, A_BYTES = COLS * 128, WARP_BYTES = 2 * X_BYTES + A_STAGES * A_BYTES;
   static constexpr int SUM_BYTES = (kShrinkWarps * ROWS * LD + ROWS * COLS) * 4;   // take the place of the rings
   static constexpr int SMEM_BYTES = 1024 + kShrinkWarps * WARP_BYTES;
   static_assert(SUM_BYTES <= kShrinkWarps * WARP_BYTES && SMEM_BYTES <= 231424, "shared memory budget");
@@ -324,16 +325,16 @@ lora_shrink_rows_kernel(const __grid_constant__ ShrinkArgs args, const __grid_co
   extern __shared__ uint8_t shrink_rows_raw[];
   uint8_t* smem = shrink_rows_raw + ((1024u - (smem_u32(shrink_rows_raw) & 1023u)) & 1023u);
   __shared__ int id_of[S::ROWS], slot_id[S::ROWS], slot_count;
-  __shared__ __align__(8) uint64_t bars[kShrinkWarps * 4];
+  __shared__ __align__(8) uint64_t bars[kShrinkWarps * (2 + S::A_STAGES)];
   const int warp = __shfl_sync(0xffffffffu, (int)(threadIdx.x >> 5), 0), lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
   const int rank = blockIdx.y, ranks = gridDim.y;
   const int chunk = blockIdx.z % args.chunks, problem = blockIdx.z / args.chunks;
   const ShrinkProblem& pr = args.p[problem];
   const int row0 = blockIdx.x * S::ROWS, row_end = min(args.T, row0 + S::ROWS);
   const uint32_t x_ring = smem_u32(smem) + warp * S::WARP_BYTES, a_ring = x_ring + 2 * S::X_BYTES;
-  const uint32_t x_bar = smem_u32(bars) + warp * 32, a_bar = x_bar + 16;
+  const uint32_t x_bar = smem_u32(bars) + warp * 8 * (2 + S::A_STAGES), a_bar = x_bar + 16;
   if (lane == 0) {
-    for (int i = 0; i < 4; ++i) mbar_init(x_bar + 8 * i, 1);
+    for (int i = 0; i < 2 + S::A_STAGES; ++i) mbar_init(x_bar + 8 * i, 1);
     fence_mbar_init();
   }
   if (!args.beside) pdl_wait();
@@ -351,11 +352,14 @@ lora_shrink_rows_kernel(const __grid_constant__ ShrinkArgs args, const __grid_co
   }
   __syncthreads();
   const int slots = slot_count;
+  // Row g of an MMA is row `rho` of its eight rows, for X and A alike: tiles lie in 128-byte swizzled rows (unit u of row r at
+  // u ^ (r & 7)), and in this order two neighbouring lanes' rows are read from different halves of the banks.
+  const int rho = g >> 1 | (g & 1) << 2;
   int id[MT][2];
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-    for (int h = 0; h < 2; ++h) id[mt][h] = id_of[mt * 16 + h * 8 + g];
+    for (int h = 0; h < 2; ++h) id[mt][h] = id_of[mt * 16 + h * 8 + rho];
   const int steps = (pr.K + kShrinkK - 1) / kShrinkK, per = (steps + ranks - 1) / ranks;
   const int step0 = min(steps, rank * per) + warp, step1 = min(steps, (rank + 1) * per);
   const bool issuer = elect_one();
@@ -382,24 +386,16 @@ lora_shrink_rows_kernel(const __grid_constant__ ShrinkArgs args, const __grid_co
     load_x(step0, 0);
     load_a(0);
     load_x(step0 + kShrinkWarps, 1);
-    load_a(1);
+    for (uint32_t i = 1; i < (uint32_t)S::A_STAGES; ++i) load_a(i);
   }
-  // tiles lie in 128-byte swizzled rows: unit u of row r at u ^ (r & 7); every row read here is g mod 8
-  const uint32_t unit[2] = {(uint32_t)(q ^ g) << 4, (uint32_t)((4 + q) ^ g) << 4};
-  uint32_t it = 0, item = 0;
+  const uint32_t unit[2] = {(uint32_t)(q ^ rho) << 4, (uint32_t)((4 + q) ^ rho) << 4};
+  uint32_t it = 0, ab = 0, a_phase = 0;
   for (int step = step0; step < step1 && slots > 0 && !failed; step += kShrinkWarps, ++it) {
-    const uint32_t xb = it & 1u, xs = x_ring + xb * S::X_BYTES + (uint32_t)g * 128u;
+    const uint32_t xb = it & 1u, xs = x_ring + xb * S::X_BYTES + (uint32_t)rho * 128u;
     if (!mbar_wait_warp(x_bar + 8 * xb, (it >> 1) & 1u, kRoleMma, (int)xb)) { failed = true; break; }
-    uint4 x[MT][2][2];   // [16 rows][half of k][rows 0-7, 8-15]
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int half = 0; half < 2; ++half)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) x[mt][half][h] = ld_shared_16(xs + mt * 2048 + h * 1024 + unit[half]);
-    for (int slot = 0; slot < slots; ++slot, ++item) {
-      const uint32_t ab = item & 1u, as = a_ring + ab * S::A_BYTES + (uint32_t)g * 128u;
-      if (!mbar_wait_warp(a_bar + 8 * ab, (item >> 1) & 1u, kRoleMma, 2 + (int)ab)) { failed = true; break; }
+    for (int slot = 0; slot < slots; ++slot) {
+      const uint32_t as = a_ring + ab * S::A_BYTES + (uint32_t)rho * 128u;
+      if (!mbar_wait_warp(a_bar + 8 * ab, a_phase, kRoleMma, 2 + (int)ab)) { failed = true; break; }
       uint4 w[2][NT8];
 #pragma unroll
       for (int half = 0; half < 2; ++half)
@@ -408,20 +404,22 @@ lora_shrink_rows_kernel(const __grid_constant__ ShrinkArgs args, const __grid_co
       const int a = slot_id[slot];
 #pragma unroll
       for (int mt = 0; mt < MT; ++mt) {
+        if (!__any_sync(0xffffffffu, id[mt][0] == a || id[mt][1] == a)) continue;   // none of these 16 rows
+        uint4 x[2][2];   // [half of k][rows 0-7, 8-15]
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) x[half][h] = ld_shared_16(xs + mt * 2048 + h * 1024 + unit[half]);
         // 64 k at a time in the tensor cores (which cut off low bits of a long running sum), added up in FP32
         float t[NT8][4];
 #pragma unroll
-        for (int nt = 0; nt < NT8; ++nt)
-          mma_m16n8k16_bf16_zero(t[nt], x[mt][0][0].x, x[mt][0][1].x, x[mt][0][0].y, x[mt][0][1].y, w[0][nt].x, w[0][nt].y);
+        for (int nt = 0; nt < NT8; ++nt) mma_m16n8k16_bf16_zero(t[nt], x[0][0].x, x[0][1].x, x[0][0].y, x[0][1].y, w[0][nt].x, w[0][nt].y);
 #pragma unroll
-        for (int nt = 0; nt < NT8; ++nt)
-          mma_m16n8k16_bf16(t[nt], x[mt][0][0].z, x[mt][0][1].z, x[mt][0][0].w, x[mt][0][1].w, w[0][nt].z, w[0][nt].w);
+        for (int nt = 0; nt < NT8; ++nt) mma_m16n8k16_bf16(t[nt], x[0][0].z, x[0][1].z, x[0][0].w, x[0][1].w, w[0][nt].z, w[0][nt].w);
 #pragma unroll
-        for (int nt = 0; nt < NT8; ++nt)
-          mma_m16n8k16_bf16(t[nt], x[mt][1][0].x, x[mt][1][1].x, x[mt][1][0].y, x[mt][1][1].y, w[1][nt].x, w[1][nt].y);
+        for (int nt = 0; nt < NT8; ++nt) mma_m16n8k16_bf16(t[nt], x[1][0].x, x[1][1].x, x[1][0].y, x[1][1].y, w[1][nt].x, w[1][nt].y);
 #pragma unroll
-        for (int nt = 0; nt < NT8; ++nt)
-          mma_m16n8k16_bf16(t[nt], x[mt][1][0].z, x[mt][1][1].z, x[mt][1][0].w, x[mt][1][1].w, w[1][nt].z, w[1][nt].w);
+        for (int nt = 0; nt < NT8; ++nt) mma_m16n8k16_bf16(t[nt], x[1][0].z, x[1][1].z, x[1][0].w, x[1][1].w, w[1][nt].z, w[1][nt].w);
 #pragma unroll
         for (int h = 0; h < 2; ++h)
           if (id[mt][h] == a) {
@@ -432,12 +430,13 @@ lora_shrink_rows_kernel(const __grid_constant__ ShrinkArgs args, const __grid_co
             }
           }
       }
-      // The products above were issued, so every fragment had arrived in its register: the tiles may be
-      // overwritten.  (Asked for right behind the reads, a tile could land before a read that was still queued.)
+      // Every fragment read above went into a product that was issued, so it had arrived in its register: the tile
+      // may be overwritten.  (Asked for right behind the reads, a tile could land before a read that was still queued.)
       __syncwarp();
       load_a(ab);
-      if (slot == 0) load_x(step + 2 * kShrinkWarps, xb);
+      if (++ab == (uint32_t)S::A_STAGES) { ab = 0; a_phase ^= 1u; }
     }
+    if (!failed) load_x(step + 2 * kShrinkWarps, xb);   // the same holds for the X tile
   }
   if (failed || aborted()) {   // copies in flight land before shared memory goes away
     const unsigned long long t0 = globaltimer_ns();
@@ -450,10 +449,12 @@ lora_shrink_rows_kernel(const __grid_constant__ ShrinkArgs args, const __grid_co
   for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      float* dst = warp_sums + (warp * S::ROWS + mt * 16 + h * 8 + g) * S::LD + 2 * q;
+      float* dst = warp_sums + (warp * S::ROWS + mt * 16 + h * 8 + rho) * S::LD + q;   // columns 2q, 2q + 1 of the MMA: ranks q, q + 4
 #pragma unroll
-      for (int nt = 0; nt < NT8; ++nt)
-        *reinterpret_cast<float2*>(dst + nt * 8) = make_float2(acc[mt][nt][2 * h], acc[mt][nt][2 * h + 1]);
+      for (int nt = 0; nt < NT8; ++nt) {
+        dst[nt * 8] = acc[mt][nt][2 * h];
+        dst[nt * 8 + 4] = acc[mt][nt][2 * h + 1];
+      }
     }
   __syncthreads();
   const int elems = (row_end - row0) * S::COLS;
@@ -532,8 +533,13 @@ struct GradArgs {
   GradProblem p[2];
   const int32_t* perm;
   const int32_t* start;
-  int n, R, block_tokens;
+  int n, R, blocks;   // blocks: of tokens (gridDim.y of lora_grad_kernel)
 };
+// Tokens per block, from the number of tokens that have an adapter (known on the device): whole steps of 32 from there on.
+__device__ __forceinline__ int grad_block_tokens(int total, int blocks) {
+  const int b = (total + blocks - 1) / blocks;
+  return b > 32 ? (b + 31) / 32 * 32 : max(4, (b + 3) / 4 * 4);
+}
 constexpr int kGradCols = 128, kGradTokens = 32, kGradStages = 3, kGradThreads = 128;
 constexpr int kGradRows = 8;   // steps whose row indices are held: more than the stages, so that no reader is overtaken
 
@@ -572,7 +578,8 @@ lora_grad_kernel(const __grid_constant__ GradArgs args) {
   pdl_wait();
   pdl_launch_dependents();
   const int total = args.start[args.n];
-  const int lo = blockIdx.y * args.block_tokens, hi = min(total, lo + args.block_tokens);
+  const int block_tokens = grad_block_tokens(total, args.blocks);
+  const int lo = blockIdx.y * block_tokens, hi = min(total, lo + block_tokens);
   if (lo >= hi) return;
   // the adapter that position `lo` belongs to: the last one that starts at or before it
   int a0 = 0, a1 = args.n - 1;
@@ -726,7 +733,8 @@ lora_join_kernel(const __grid_constant__ GradArgs args) {
   pdl_wait();
   pdl_launch_dependents();
   const int s0 = args.start[a], s1 = args.start[a + 1];
-  const int b0 = s0 / args.block_tokens, b1 = (s1 - 1) / args.block_tokens;
+  const int block_tokens = grad_block_tokens(args.start[args.n], args.blocks);
+  const int b0 = s0 / block_tokens, b1 = (s1 - 1) / block_tokens;
   if (s1 > s0 && b0 == b1) return;
   const int64_t elems = (int64_t)args.R * pr.cols;   // a multiple of 8
   for (int64_t e = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 4; e < elems; e += (int64_t)gridDim.x * 1024) {

@@ -106,7 +106,10 @@ static int make_map_3d(CUtensorMap* map, CUtensorMapDataType dt, int elem_bytes,
   cuuint32_t box[3] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows, 1};
   cuuint32_t estr[3] = {1, 1, 1};
   CUresult r = fn(map, dt, 3, const_cast<void*>(ptr), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  // Rows that start anywhere in a 64-byte piece make every 128-byte box row straddle two lines, and with
+                  // 256-byte promotion two pairs of them: us at 256 / 128 bytes, pitch 2832 bytes 2048 x 1416 x 32768
+                  // 205 / 169, pitch 5680 bytes 128 x 2840 x 100000 162 / 140; at pitch 5696 and 2880 no difference.
+                  ld * elem_bytes % 64 == 0 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS)
     return fail(GEMM_B200_ERR_CUDA,
                 "cuTensorMapEncodeTiled failed with CUresult %d (rows=%lld cols=%lld ld=%lld batch=%lld stride=%lld box=%dx%d)",
@@ -353,11 +356,6 @@ static int launch_splitk_reduce(const float* scratch, int64_t M, int64_t N, int 
   return GEMM_B200_OK;
 }
 
-// A product whose A has fewer rows than this streams B slowly: the loads of 128-row boxes with fewer than 16
-// rows inside the matrix hold up the ring (131072 x 4096 bf16 B, 128-column tiles: 1 row 239 us, 15 rows 233,
-// 16 rows 166, 64 rows 169).  Operators with scratch of their own give A that many rows.
-constexpr int64_t kMinMapRows = 16;
-
 struct Bf16Args {
   const void *A, *B;
   void* C;
@@ -367,8 +365,6 @@ struct Bf16Args {
   int64_t batch = 1, stride_a = 0, stride_b = 0, stride_c = 0;
   // split-K (FP32 output only): C is then the scratch [k_splits][M][N], ldc = N
   int k_splits = 1;
-  // rows of A in memory where there are more than M (plain layout, one problem; see kMinMapRows); 0: M
-  int64_t a_rows = 0;
 };
 
 // One instantiation per (config, B layout, output type); A_MN: A is stored transposed, [K, M] row-major;
@@ -389,8 +385,8 @@ static int launch_bf16_fused(const Bf16Args& a, const Fuse& fuse) {
                              CU_TENSOR_MAP_SWIZZLE_128B))
       return rc;
   } else {
-    if (int rc = make_map_3d(&tmA, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.A, a.a_rows ? a.a_rows : a.M, a.K, a.lda, za,
-                             a.a_rows ? a.a_rows * a.lda : sa, kBlockK, kBlockM, CU_TENSOR_MAP_SWIZZLE_128B))
+    if (int rc = make_map_3d(&tmA, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a.A, a.M, a.K, a.lda, za, sa, kBlockK, Cfg::A_ROWS,
+                             CU_TENSOR_MAP_SWIZZLE_128B))
       return rc;
   }
   if (B_MN) {
@@ -422,6 +418,8 @@ static int launch_bf16_fused(const Bf16Args& a, const Fuse& fuse) {
   shape.K = (int)a.K;
   shape.tiles_m = (int)ceil_div64(a.M, kBlockM * CG);
   shape.tiles_n = (int)ceil_div64(a.N, Cfg::TILE_N);
+  if (Cfg::A_ROWS != kBlockM && a.M > Cfg::A_ROWS)
+    return fail(GEMM_B200_ERR_INVALID_ARG, "gemm_bf16: this variant handles at most %d rows of A", Cfg::A_ROWS);
   const int num_kb = (int)ceil_div64(a.K, kBlockK);
   if (a.k_splits > 1 && !(OUT_F32 && a.batch == 1))
     return fail(GEMM_B200_ERR_INVALID_ARG, "gemm_bf16: K splits need FP32 output and one problem");

@@ -86,36 +86,16 @@ xent_finish_kernel(const float2* __restrict__ part, const float* __restrict__ la
   loss[out] = label < 0 ? 0.f : (label >= V ? NAN : total - label_logit[out]);
 }
 
-// X with its last rows zero, for products of fewer rows than a tensor map streams well with (kMinMapRows).
-__global__ void __launch_bounds__(128)
-xent_pad_kernel(const __nv_bfloat16* __restrict__ X, int64_t ldx, __nv_bfloat16* __restrict__ Xp, int64_t ldp, int T, int D) {
-  const int64_t row = blockIdx.x;
-  pdl_wait();
-  pdl_launch_dependents();
-  for (int i = threadIdx.x * 8; i < D; i += 128 * 8) {
-    if (i + 8 <= D) {
-      *reinterpret_cast<uint4*>(Xp + row * ldp + i) = row < T ? *reinterpret_cast<const uint4*>(X + row * ldx + i) : make_uint4(0u, 0u, 0u, 0u);
-    } else {
-      for (int j = i; j < D; ++j) Xp[row * ldp + j] = row < T ? X[row * ldx + j] : __float2bfloat16_rn(0.f);
-    }
-  }
-}
-
 // One block per row: the numbers the gradient epilogue needs, and the row of X for the product d^T X with
 // rows of weight zero (padding, whatever it holds) as zeros, since 0 * NaN would reach every row of dW.
 __global__ void __launch_bounds__(128)
 xent_prepare_kernel(const int64_t* __restrict__ labels, const float* __restrict__ lse, const float* __restrict__ grad_loss,
                     int64_t grad_loss_stride, const float* __restrict__ grad_lse, int64_t grad_lse_stride,
-                    const __nv_bfloat16* __restrict__ X, int64_t ldx, XentRow* __restrict__ rows, __nv_bfloat16* __restrict__ Xw, int T,
-                    int D, int V) {
+                    const __nv_bfloat16* __restrict__ X, int64_t ldx, XentRow* __restrict__ rows, __nv_bfloat16* __restrict__ Xw, int D,
+                    int V) {
   const int64_t row = blockIdx.x;
   pdl_wait();
   pdl_launch_dependents();
-  uint4* dst = reinterpret_cast<uint4*>(Xw + row * D);
-  if (row >= T) {   // rows up to kMinMapRows
-    for (int i = threadIdx.x; i < D / 8; i += 128) dst[i] = make_uint4(0u, 0u, 0u, 0u);
-    return;
-  }
   const int64_t label = labels[row];
   float g = label < 0 ? 0.f : grad_loss[row * grad_loss_stride];
   if (label >= V) g = NAN;
@@ -130,6 +110,7 @@ xent_prepare_kernel(const int64_t* __restrict__ labels, const float* __restrict_
     rows[row] = r;
   }
   const uint4* src = reinterpret_cast<const uint4*>(X + row * ldx);
+  uint4* dst = reinterpret_cast<uint4*>(Xw + row * D);
   for (int i = threadIdx.x; i < D / 8; i += 128) dst[i] = live ? src[i] : make_uint4(0u, 0u, 0u, 0u);
 }
 

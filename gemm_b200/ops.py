@@ -315,8 +315,9 @@ def gemm_bf16_xent(X: torch.Tensor, W: torch.Tensor, labels: torch.Tensor) -> tu
     ``lse[t] = log(sum_v exp(logit[t, v]))`` and ``loss[t] = lse[t] - logit[t, labels[t]]``.  A negative label
     (padding) has loss 0; a label >= V makes its loss NaN.  Logits, maxima and sums are FP32."""
     device, T, V, D, ldx, ldw = _xent_operands(X, W, labels)
-    loss, lse = torch.empty((2, T), device=device, dtype=torch.float32)
-    nbytes = lib.gemm_b200_gemm_bf16_xent_scratch_bytes(T, V, D)
+    loss = torch.empty(T, device=device, dtype=torch.float32)
+    lse = torch.empty(T, device=device, dtype=torch.float32)
+    nbytes = lib.gemm_b200_gemm_bf16_xent_scratch_bytes(T, V)
     scratch = _scratch(nbytes, device)
     with _OnDevice(device):
         check(lib.gemm_b200_gemm_bf16_xent(X.data_ptr(), W.data_ptr(), labels.data_ptr(), loss.data_ptr(), lse.data_ptr(), T, V, D, ldx, ldw,
@@ -398,7 +399,7 @@ def gemm_bf16_lora(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.T
         ldy = _out_matrix(out, device, out_dtype, T, N)
     od = _lib.OUT_F32 if out_dtype == torch.float32 else _lib.OUT_BF16
     with _OnDevice(device):
-        nbytes = lib.gemm_b200_gemm_bf16_lora_scratch_bytes(T, N, D, R, od)
+        nbytes = lib.gemm_b200_gemm_bf16_lora_scratch_bytes(T, N, D, R, n, od)
         scratch = _scratch(nbytes, device)
         check(lib.gemm_b200_gemm_bf16_lora(
             X.data_ptr(), W.data_ptr(), A.data_ptr(), B.data_ptr(), ids.data_ptr(), scale_ptr, out.data_ptr(), T, N, D, R, n, ldx, ldw, lda, sa,

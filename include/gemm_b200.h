@@ -188,7 +188,7 @@ int gemm_b200_gemm_bf16_grouped(const void* A, const void* B, void* C, int64_t g
 int gemm_b200_gemm_bf16_xent(const void* X, const void* W, const int64_t* labels, float* loss, float* lse,
                              int64_t T, int64_t V, int64_t D, int64_t ldx, int64_t ldw,
                              void* scratch, size_t scratch_bytes, void* stream);
-size_t gemm_b200_gemm_bf16_xent_scratch_bytes(int64_t T, int64_t V, int64_t D);
+size_t gemm_b200_gemm_bf16_xent_scratch_bytes(int64_t T, int64_t V);
 
 /* Its gradient, with lse as the call above wrote it:
  *   d_tv = (g_t + h_t) exp(z_tv - lse_t) - g_t [v == labels[t]],   dX = d W,   dW = d^T X   (bf16)
@@ -223,7 +223,7 @@ int gemm_b200_gemm_bf16_lora(const void* X, const void* W, const void* A, const 
                              const float* scales, void* Y, int64_t T, int64_t N, int64_t D, int64_t R, int64_t adapters,
                              int64_t ldx, int64_t ldw, int64_t lda, int64_t stride_a, int64_t ldb, int64_t stride_b,
                              int64_t ldy, int w_layout, int out_dtype, void* scratch, size_t scratch_bytes, void* stream);
-size_t gemm_b200_gemm_bf16_lora_scratch_bytes(int64_t T, int64_t N, int64_t D, int64_t R, int out_dtype);
+size_t gemm_b200_gemm_bf16_lora_scratch_bytes(int64_t T, int64_t N, int64_t D, int64_t R, int64_t adapters, int out_dtype);
 
 /* Gradients of the adapters for the output gradient dY[T,N]:
  *   dA_a = scales[a] * sum_{t: ids[t] = a} (dY[t] B_a^T)^T X[t],   dB_a = scales[a] * sum (X[t] A_a^T)^T dY[t]

@@ -81,10 +81,10 @@ def test_lora_grad_refusals(kw, code):
 
 
 def test_scratch_of_nothing_is_nothing():
-    assert L.gemm_b200_gemm_bf16_xent_scratch_bytes(0, 100, 64) == 0
-    assert L.gemm_b200_gemm_bf16_xent_scratch_bytes(300, 1000, 64) >= 4 * 300 * 8 + 300 * 4
+    assert L.gemm_b200_gemm_bf16_xent_scratch_bytes(0, 100) == 0
+    assert L.gemm_b200_gemm_bf16_xent_scratch_bytes(300, 1000) >= 4 * 300 * 8 + 300 * 4
     assert L.gemm_b200_gemm_bf16_xent_grad_scratch_bytes(0, 100, 64) == 0
-    assert L.gemm_b200_gemm_bf16_lora_scratch_bytes(0, 64, 64, 8, 0) == 0
+    assert L.gemm_b200_gemm_bf16_lora_scratch_bytes(0, 64, 64, 8, 2, 0) == 0
     assert L.gemm_b200_gemm_bf16_lora_grad_scratch_bytes(4, 64, 64, 0, 2, 0) == 0
 
 
