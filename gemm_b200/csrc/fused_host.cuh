@@ -130,18 +130,21 @@ static int xent_sizes(const char* who, int64_t T, int64_t V, int64_t D, int64_t 
 constexpr int64_t kXentPieceBytes = 256ll << 20;
 
 struct XentGradPlan {
+  int halves;                 // bf16 summands of d, one below the other: two for up to 64 rows, one row tile (xent.cuh)
   int64_t pieces, piece;      // columns of the vocabulary per piece (the last may be shorter)
   int dx_splits, dw_splits;   // K ranges of the products dX = d W (K: the piece) and dW = d^T X (K: the tokens)
-  bool dx_acc;                // dX is summed in FP32 slices: more than one piece, or K ranges
+  bool dx_acc;                // dX is summed in FP32 slices: more than one piece, K ranges, or two halves
   XentGradPlan(int64_t T, int64_t V, int64_t D, int sms) {
-    int64_t most = kXentPieceBytes / (2 * (T > 0 ? T : 1)) / kBlockN * kBlockN;
+    halves = 2 * T <= kBlockM ? 2 : 1;
+    const int64_t rows = halves * T;
+    int64_t most = kXentPieceBytes / (2 * (rows > 0 ? rows : 1)) / kBlockN * kBlockN;
     if (most < 2 * kBlockN) most = 2 * kBlockN;
     pieces = ceil_div64(V, most);
     piece = pieces == 1 ? V : ceil_div64(ceil_div64(V, pieces), kBlockN) * kBlockN;
     pieces = ceil_div64(V, piece);
-    dx_splits = bf16_auto_splits(T, D, piece, sms);
-    dw_splits = bf16_auto_splits(piece, D, T, sms);
-    dx_acc = pieces > 1 || dx_splits > 1;
+    dx_splits = bf16_auto_splits(rows, D, piece, sms);
+    dw_splits = bf16_auto_splits(piece, D, rows, sms);
+    dx_acc = pieces > 1 || dx_splits > 1 || halves > 1;
   }
 };
 struct XentGradScratch {
@@ -154,9 +157,9 @@ struct XentGradScratch {
     Carver c{static_cast<char*>(base)};
     ldd = ceil_div64(p.piece, 8) * 8;
     rows = c.take<XentRow>(T);
-    xw = c.take<__nv_bfloat16>(T * D);
-    d = c.take<__nv_bfloat16>(T * ldd);
-    dx = c.take<float>(p.dx_acc ? (int64_t)p.dx_splits * T * D : 0);
+    xw = c.take<__nv_bfloat16>(p.halves * T * D);
+    d = c.take<__nv_bfloat16>(p.halves * T * ldd);
+    dx = c.take<float>(p.dx_acc ? (int64_t)p.dx_splits * p.halves * T * D : 0);
     dw = c.take<float>(p.dw_splits > 1 ? (int64_t)p.dw_splits * p.piece * D : 0);
     bytes = c.used;
   }
@@ -232,7 +235,7 @@ static int xent_grad_entry(const void* X, const void* W, const int64_t* labels, 
     fprintf(stderr, "[gemm_b200] gemm_bf16_xent_grad T=%lld V=%lld D=%lld -> %lld pieces of %lld, K ranges %d (dX) %d (dW)\n", (long long)T,
             (long long)V, (long long)D, (long long)plan.pieces, (long long)plan.piece, plan.dx_splits, plan.dw_splits);
   if (int rc = launch_plain(xent_prepare_kernel, dim3((unsigned)T), 128, 0, 1, st, labels, lse, grad_loss, grad_loss_stride, grad_lse,
-                            grad_lse_stride, static_cast<const __nv_bfloat16*>(X), ldx, ws.rows, ws.xw, (int)D, (int)V))
+                            grad_lse_stride, static_cast<const __nv_bfloat16*>(X), ldx, ws.rows, ws.xw, plan.halves, (int)D, (int)V))
     return rc;
   int dx_slices = 1;
   for (int64_t v0 = 0; v0 < V; v0 += plan.piece) {
@@ -240,14 +243,21 @@ static int xent_grad_entry(const void* X, const void* W, const int64_t* labels, 
     const char* Wp = static_cast<const char*>(W) + v0 * ldw * 2;
     // d of the piece
     const Bf16Args z{X, Wp, ws.d, T, n, D, ldx, ldw, ws.ldd, st};
-    const XentGradFuse fuse{ws.rows, (int)v0};
+    XentGradFuse fuse = {};
+    fuse.rows = ws.rows;
+    fuse.col0 = (int)v0;
+    fuse.low = plan.halves > 1;
     int rc;
+    if (fuse.low && (rc = make_map_3d(&fuse.tmLow, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ws.d + T * ws.ldd, T, n, ws.ldd, 1, T * ws.ldd, 64, 32,
+                                      CU_TENSOR_MAP_SWIZZLE_128B)))   // the box of the epilogue's stores
+      return rc;
     if (T <= kBlockM) rc = launch_row_tile<false, false>(z, fuse);
     else if (bf16_pairs_dynamic(T, n, D, di.sms)) rc = launch_bf16_fused<Bf16_2cta_tma_m_dyn, false, false>(z, fuse);
     else rc = launch_bf16_fused<Bf16_2cta_tma_m, false, false>(z, fuse);
     if (rc) return rc;
     // dX (+)= d W
-    Bf16Args gx{ws.d, Wp, dX, T, D, n, ws.ldd, ldw, lddx, st};
+    const int64_t rows = plan.halves * T;
+    Bf16Args gx{ws.d, Wp, dX, rows, D, n, ws.ldd, ldw, lddx, st};
     if (!plan.dx_acc && T <= kBlockM) {
       rc = launch_row_tile<true, false>(gx, NoFuse());
     } else if (!plan.dx_acc) {
@@ -266,21 +276,22 @@ static int xent_grad_entry(const void* X, const void* W, const int64_t* labels, 
     }
     if (rc) return rc;
     // dW of the piece's rows = d^T X
-    Bf16Args gw{ws.d, ws.xw, static_cast<char*>(dW) + v0 * lddw * 2, n, D, T, ws.ldd, D, lddw, st};
+    Bf16Args gw{ws.d, ws.xw, static_cast<char*>(dW) + v0 * lddw * 2, n, D, rows, ws.ldd, D, lddw, st};
     if (plan.dw_splits > 1) {
       rc = launch_bf16_splitk(gw, GEMM_B200_B_ROW_MAJOR_KN, GEMM_B200_OUT_BF16, plan.dw_splits, ws.dw, /*a_mn=*/true);
     } else {
       // A K of a few blocks: the store of dW bounds the product, and single CTAs (two per pair to drain
       // accumulators) store faster (dW [32001, 2048] of 67 tokens 36 us against 45, [131072, 4096] of 16 190
       // against 286); from 512 tokens on pairs are as fast ([50001, 1024] of 509 tokens 51 / 49).
-      const int config = T <= 256 ? (int)kBf16Cfg1cta : pick_bf16_config(n, D, T, di.sms);
+      const int config = rows <= 256 ? (int)kBf16Cfg1cta : pick_bf16_config(n, D, rows, di.sms);
       rc = GEMM_B200_ERR_UNSUPPORTED;
       for (const Bf16AtEntry& e : kBf16AtConfigs)
         if (e.config == config) rc = e.launch[GEMM_B200_B_ROW_MAJOR_KN][GEMM_B200_OUT_BF16](gw);
     }
     if (rc) return rc;
   }
-  if (plan.dx_acc) return launch_splitk_reduce(ws.dx, T, D, dx_slices, dX, lddx, GEMM_B200_OUT_BF16, st);
+  // slice i of half h starts at row (2 i + h) T of the scratch: twice as many slices of T rows
+  if (plan.dx_acc) return launch_splitk_reduce(ws.dx, T, D, plan.halves * dx_slices, dX, lddx, GEMM_B200_OUT_BF16, st);
   return GEMM_B200_OK;
 }
 
@@ -290,8 +301,12 @@ static int xent_grad_entry(const void* X, const void* W, const int64_t* labels, 
 constexpr int64_t kLoraMaxRank = 128;
 
 static int lora_rp(int64_t R) { return R <= 16 ? 16 : R <= 32 ? 32 : R <= 64 ? 64 : 128; }
-// bf16 summands per value of V: FP32 results keep 24 bits of it, bf16 results the 8 they are rounded to themselves
-static int lora_terms(int out_dtype) { return out_dtype == GEMM_B200_OUT_F32 ? 3 : 1; }
+// bf16 summands per value of V: FP32 results keep 24 bits of it, bf16 results the 8 they are rounded to themselves.  With
+// few rows and a low rank these roundings do not average out (one row, rank 1: one of them is the whole
+// error of the adapter's term), and there the summands cost nothing: three fit into the K block of one.
+static int lora_terms(int64_t T, int64_t R, int out_dtype) { return out_dtype == GEMM_B200_OUT_F32 || (T <= 64 && R <= 16) ? 3 : 1; }
+// the gradient's: with few tokens its time is that of its launches
+static int lora_grad_terms(int64_t T, int out_dtype) { return out_dtype == GEMM_B200_OUT_F32 || T <= 64 ? 3 : 1; }
 
 static int lora_sizes(const char* who, int64_t T, int64_t N, int64_t D, int64_t R, int64_t n, int64_t ldx, int64_t lda, int64_t stride_a,
                       int64_t ldb, int64_t stride_b, int out_dtype) {
@@ -438,7 +453,7 @@ static int lora_entry(const void* X, const void* W, const void* A, const void* B
     return fail(GEMM_B200_ERR_ALIGNMENT, "gemm_bf16_lora: X, W, A, B and Y must be 16-byte aligned, ldw a multiple of 8, ldy*sizeof(Y) of 16 bytes");
   DeviceInfo di;
   if (int rc = check_blackwell("gemm_bf16_lora", &di)) return rc;
-  const int terms = lora_terms(out_dtype), rp = lora_rp(R), splits = lora_splits(T, N, D, R, n, terms, di.sms);
+  const int terms = lora_terms(T, R, out_dtype), rp = lora_rp(R), splits = lora_splits(T, N, D, R, n, terms, di.sms);
   const LoraScratch ws(scratch, T, N, R, terms, splits);
   if (int rc = check_scratch("gemm_bf16_lora", scratch, scratch_bytes, ws.bytes)) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
@@ -520,9 +535,8 @@ struct LoraGradScratch {
   }
 };
 
-template <int MT, int TERMS>
+template <int MT, int TERMS, bool F32>
 static int launch_lora_grad(const GradArgs& ga, const LoraGradPlan& plan, const DeviceInfo& di, cudaStream_t st) {
-  constexpr bool F32 = TERMS > 1;
   auto kern = lora_grad_kernel<MT, TERMS, F32>;
   constexpr int smem = GradShape<MT, TERMS>::SMEM_BYTES;
   if (int rc = allow_smem(kern, smem, di)) return rc;
@@ -533,6 +547,14 @@ static int launch_lora_grad(const GradArgs& ga, const LoraGradPlan& plan, const 
   int64_t bx = ceil_div64(8 * (int64_t)di.sms, 2 * (int64_t)ga.n);
   if (bx > most) bx = most;
   return launch_plain(lora_join_kernel<F32>, dim3((unsigned)bx, (unsigned)ga.n, 2), 256, 0, 1, st, ga);
+}
+
+template <int TERMS, bool F32>
+static int launch_lora_grad_rp(int rp, const GradArgs& ga, const LoraGradPlan& plan, const DeviceInfo& di, cudaStream_t st) {
+  return rp == 16   ? launch_lora_grad<1, TERMS, F32>(ga, plan, di, st)
+         : rp == 32 ? launch_lora_grad<2, TERMS, F32>(ga, plan, di, st)
+         : rp == 64 ? launch_lora_grad<4, TERMS, F32>(ga, plan, di, st)
+                    : launch_lora_grad<8, TERMS, F32>(ga, plan, di, st);
 }
 
 static int lora_grad_entry(const void* X, const void* dY, const void* A, const void* B, const int32_t* ids, const float* scales, void* dA,
@@ -554,7 +576,7 @@ static int lora_grad_entry(const void* X, const void* dY, const void* A, const v
   }
   DeviceInfo di;
   if (int rc = check_blackwell("gemm_bf16_lora_grad", &di)) return rc;
-  const int terms = lora_terms(out_dtype), rp = lora_rp(R);
+  const int terms = lora_grad_terms(T, out_dtype), rp = lora_rp(R);
   const LoraGradPlan plan(T, N, D, R, terms, di.sms);
   const LoraGradScratch ws(scratch, T, N, D, R, n, terms, plan);
   if (int rc = check_scratch("gemm_bf16_lora_grad", scratch, scratch_bytes, ws.bytes)) return rc;
@@ -581,11 +603,8 @@ static int lora_grad_entry(const void* X, const void* dY, const void* A, const v
   ga.n = (int)n;
   ga.R = (int)R;
   ga.blocks = (int)plan.blocks;
-  if (terms == 1)
-    return rp == 16 ? launch_lora_grad<1, 1>(ga, plan, di, st) : rp == 32 ? launch_lora_grad<2, 1>(ga, plan, di, st)
-         : rp == 64 ? launch_lora_grad<4, 1>(ga, plan, di, st) : launch_lora_grad<8, 1>(ga, plan, di, st);
-  return rp == 16 ? launch_lora_grad<1, 3>(ga, plan, di, st) : rp == 32 ? launch_lora_grad<2, 3>(ga, plan, di, st)
-       : rp == 64 ? launch_lora_grad<4, 3>(ga, plan, di, st) : launch_lora_grad<8, 3>(ga, plan, di, st);
+  if (out_dtype == GEMM_B200_OUT_F32) return launch_lora_grad_rp<3, true>(rp, ga, plan, di, st);
+  return terms > 1 ? launch_lora_grad_rp<3, false>(rp, ga, plan, di, st) : launch_lora_grad_rp<1, false>(rp, ga, plan, di, st);
 }
 
 static int current_sms() {
@@ -621,7 +640,7 @@ extern "C" size_t gemm_b200_gemm_bf16_lora_scratch_bytes(int64_t T, int64_t N, i
   using namespace gemm_b200::tc;
   const int sms = current_sms();
   if (T <= 0 || N <= 0 || D <= 0 || R <= 0 || R > kLoraMaxRank || adapters <= 0 || sms <= 0) return 0;
-  const int terms = lora_terms(out_dtype);
+  const int terms = lora_terms(T, R, out_dtype);
   return LoraScratch(nullptr, T, N, R, terms, lora_splits(T, N, D, R, adapters, terms, sms)).bytes;
 }
 extern "C" int gemm_b200_gemm_bf16_lora(const void* X, const void* W, const void* A, const void* B, const int32_t* ids, const float* scales,
@@ -635,7 +654,8 @@ extern "C" size_t gemm_b200_gemm_bf16_lora_grad_scratch_bytes(int64_t T, int64_t
   using namespace gemm_b200::tc;
   const int sms = current_sms();
   if (T <= 0 || N <= 0 || D <= 0 || R <= 0 || R > kLoraMaxRank || adapters <= 0 || sms <= 0) return 0;
-  return LoraGradScratch(nullptr, T, N, D, R, adapters, lora_terms(out_dtype), LoraGradPlan(T, N, D, R, lora_terms(out_dtype), sms)).bytes;
+  const int terms = lora_grad_terms(T, out_dtype);
+  return LoraGradScratch(nullptr, T, N, D, R, adapters, terms, LoraGradPlan(T, N, D, R, terms, sms)).bytes;
 }
 extern "C" int gemm_b200_gemm_bf16_lora_grad(const void* X, const void* dY, const void* A, const void* B, const int32_t* ids,
                                              const float* scales, void* dA, void* dB, int64_t T, int64_t N, int64_t D, int64_t R,

@@ -237,8 +237,10 @@ struct XentRow {
 };
 struct XentGradFuse {
   static constexpr FuseKind KIND = kFuseXentGrad;
+  CUtensorMap tmLow;        // [M, N] like C: what the rounding of d to bf16 cuts off, rounded in turn; only with `low`
   const XentRow* rows;      // [M]
   int col0;                 // vocabulary index of column 0 of this launch
+  int low;
 };
 
 // Low-rank adapters beside the projection:  C[t] += V[t] @ Ad_a,  a = ids[t]  (no term for a < 0).
@@ -847,6 +849,10 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
         (void)xr;
         constexpr int SLABS = (Cfg::ACC_KB > 0 ? 128 : BN) / SLAB_COLS;
         static_assert(Cfg::ACC_KB == 0 || OUT_F32, "accumulators are drained for FP32 results");
+        int parts = 1;   // the gradient of few rows leaves in two bf16 summands, one after the other
+        if constexpr (Fuse::KIND == kFuseXentGrad) parts = fuse.low ? 2 : 1;
+#pragma unroll 1
+        for (int part = 0; part < parts; ++part)
 #pragma unroll(Cfg::ACC_KB > 0 ? SLABS : 1)
         for (int c = 0; c < SLABS; ++c, ++store_it) {
           const uint32_t buf = stage0 + (store_it % Cfg::EPI_BUFS) * Cfg::EPI_WARP_BUF;
@@ -888,6 +894,13 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
                   for (int j = 0; j < 32; ++j)
                     if (j == at) v[j] = __float_as_uint(__uint_as_float(v[j]) - xr.b);
                 }
+                if (part) {
+#pragma unroll
+                  for (int j = 0; j < 32; ++j) {
+                    const float d = __uint_as_float(v[j]);
+                    v[j] = __float_as_uint(d - __bfloat162float(__float2bfloat16_rn(d)));
+                  }
+                }
               }
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
@@ -910,6 +923,8 @@ gemm_bf16_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant_
           if (lane == 0) {
             if constexpr (Fuse::KIND == kFuseAdd) {
               if (m0 < shape.M && x < shape.N) tma_add_f32_3d(&tmC, x, m0, shape.k_splits > 1 ? split : bi, buf);
+            } else if constexpr (Fuse::KIND == kFuseXentGrad) {
+              if (m0 < shape.M && x < shape.N) tma_store_3d(part ? &fuse.tmLow : &tmC, x, m0, 0, buf);
             } else if (m0 < shape.M && x < shape.N) tma_store_3d(&tmC, x, m0, shape.k_splits > 1 ? split : bi, buf);   // split-K: slice `split` of the scratch
             tma_store_commit();
           }

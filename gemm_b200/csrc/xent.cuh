@@ -5,9 +5,12 @@
 //
 // with g, h the gradients of loss and lse.  z is never kept: the forward pass reduces it in the epilogue of the
 // product (XentStatsFuse in gemm_bf16.cuh) to one (maximum, sum) pair per row and 128 columns, and the gradient recomputes it a piece of the vocabulary at a time, turning the accumulators
-// into d in the epilogue (XentGradFuse).  d is rounded to bf16 once, because the two products behind it
-// take bf16 operands; it is a relative rounding of each value (2^-9), of the size of the rounding of the
-// results themselves.
+// into d in the epilogue (XentGradFuse).  d is rounded to bf16, because the two products behind it take bf16
+// operands: a relative rounding of each value (2^-9 at most), of the size of the rounding of the results
+// themselves and independent from value to value.  With few rows one of these roundings, that of the label's
+// entry, is most of a row's error, so up to 64 rows are kept as two bf16 summands (16 bits), one below
+// the other: rows T + t of d for dX = d W, whose two halves are added in FP32, and tokens T + t for dW = d^T X.  W is
+// still read once and dW written once, which is what bounds these sizes.
 //
 // The reference has no loss; the products extend its operator (naive/naive.cpp:6-22).
 #pragma once
@@ -91,8 +94,8 @@ xent_finish_kernel(const float2* __restrict__ part, const float* __restrict__ la
 __global__ void __launch_bounds__(128)
 xent_prepare_kernel(const int64_t* __restrict__ labels, const float* __restrict__ lse, const float* __restrict__ grad_loss,
                     int64_t grad_loss_stride, const float* __restrict__ grad_lse, int64_t grad_lse_stride,
-                    const __nv_bfloat16* __restrict__ X, int64_t ldx, XentRow* __restrict__ rows, __nv_bfloat16* __restrict__ Xw, int D,
-                    int V) {
+                    const __nv_bfloat16* __restrict__ X, int64_t ldx, XentRow* __restrict__ rows, __nv_bfloat16* __restrict__ Xw, int copies,
+                    int D, int V) {
   const int64_t row = blockIdx.x;
   pdl_wait();
   pdl_launch_dependents();
@@ -110,8 +113,10 @@ xent_prepare_kernel(const int64_t* __restrict__ labels, const float* __restrict_
     rows[row] = r;
   }
   const uint4* src = reinterpret_cast<const uint4*>(X + row * ldx);
-  uint4* dst = reinterpret_cast<uint4*>(Xw + row * D);
-  for (int i = threadIdx.x; i < D / 8; i += 128) dst[i] = live ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+  for (int c = 0; c < copies; ++c) {   // one below the other: [copies][T][D]
+    uint4* dst = reinterpret_cast<uint4*>(Xw + (row + (int64_t)c * gridDim.x) * D);
+    for (int i = threadIdx.x; i < D / 8; i += 128) dst[i] = live ? src[i] : make_uint4(0u, 0u, 0u, 0u);
+  }
 }
 
 }  // namespace tc
