@@ -333,12 +333,12 @@ static int shrink_cluster(int64_t blocks, int64_t max_k, int64_t places) {
 
 template <int NT8>
 static int launch_shrink_few(ShrinkArgs args, int problems, int64_t max_k, const DeviceInfo& di, cudaStream_t st) {
-  using S = ShrinkShape<1, NT8>;
-  auto kern = lora_shrink_kernel<1, NT8>;
+  using S = ShrinkShape<NT8>;
+  auto kern = lora_shrink_kernel<NT8>;
   if (int rc = allow_smem(kern, S::SMEM_BYTES, di)) return rc;
   // a block per row, so that every adapter streams on its own; from 65 rows on four share a block (97 rows of 32
   // requests, rank 113: 32 us with sixteen, whose adapters a warp takes one after another)
-  args.rows_per_block = args.T <= 64 ? 1 : 4;
+  args.rows_per_block = args.T <= 64 ? 1 : kShrinkFewRows;
   const int64_t blocks = ceil_div64(args.T, args.rows_per_block), z = problems * args.chunks;
   const int ks = shrink_cluster(blocks * z, max_k, 4 * (int64_t)di.sms);   // rows without an adapter leave at once
   return launch_plain(kern, dim3((unsigned)blocks, (unsigned)ks, (unsigned)z), 32 * kShrinkWarps, S::SMEM_BYTES, ks, st, args);

@@ -48,15 +48,14 @@ __device__ __forceinline__ float ld_shared_cluster_f32(uint32_t cluster_addr) {
 // the rounding of the result).  Rows without an adapter are not written (nothing reads them); a row
 // with an id >= n becomes NaN.
 //
-// One block: up to 16 * MT rows and, in a cluster of gridDim.y blocks, a share of K.  Its eight warps are
-// dealt out to the distinct adapters of the rows first and to K second, so that a block of one
-// request and a block of sixteen keep the same number of loads in flight.  A warp copies 64 k at a time (whole
-// 128-byte lines of eight lanes; 64-byte pieces of four lanes ran into the SM's rate of requests: 56 us
-// instead of REPLACE_SHRINK for 8192 x 8192) into two stages of its own in shared memory with cp.async and waits for
-// nobody else.  The order of k inside a product is free, so a lane reads sixteen bytes of a row (eight
-// consecutive k) as the k pairs of two MMAs, in the same way for X and A.  A row is loaded only under its
-// own adapter.  With up to eight adapters a warp has one at most and leaves its rows' sums in its own stages, to be
-// added over the warps; with more, a row belongs to one warp alone.  Then the cluster adds up.  The order is fixed.
+// Few rows (lora_shrink_kernel): a block has up to four of them and, in a cluster of gridDim.y blocks, a share of K.  Its
+// eight warps are dealt out to the rows' adapters first and to K second, so that a block of one request and a block of
+// four keep the same number of loads in flight: these sizes are bound by the latency of few, long reads.  A warp
+// copies 64 k at a time (cp.async, a 128-byte line by eight lanes) into two stages of its own in shared memory and waits
+// for nobody else.  The order of k inside a product is free, so a lane reads sixteen bytes of a row (eight
+// consecutive k) as the k pairs of two MMAs, in the same way for X and A.  A row is loaded only under its own
+// adapter.  Every warp leaves its rows' sums in its stages; they are added over the warps and then over the cluster,
+// in a fixed order.  One row of 4096, rank 16: 6.5 us, most of it the launch and two round trips to memory.
 // ---------------------------------------------------------------------------------------
 struct ShrinkProblem {
   const __nv_bfloat16* X;
@@ -69,21 +68,21 @@ struct ShrinkArgs {
   ShrinkProblem p[2];
   const int32_t* ids;
   const float* scales;   // may be null: 1
-  int T, R, n, rp, terms, rows_per_block, chunks;   // chunks of 64 ranks
+  int T, R, n, rp, terms, chunks;   // chunks of 64 ranks
+  int rows_per_block;               // lora_shrink_kernel: at most kShrinkFewRows
   // launched behind a kernel whose output is not read here (lora_sort_kernel, which lets it be scheduled only after its own
   // wait): run beside it, and wait for it only at the end, for the kernel behind this one
   bool beside;
 };
-constexpr int kShrinkWarps = 8, kShrinkStages = 2, kShrinkK = 64, kShrinkMaxCluster = 8;
+constexpr int kShrinkWarps = 8, kShrinkK = 64, kShrinkMaxCluster = 8, kShrinkFewRows = 4;
 
-template <int MT, int NT8>
+template <int NT8>
 struct ShrinkShape {
-  static constexpr int ROWS = 16 * MT, COLS = 8 * NT8, LD = COLS + 8;
-  static constexpr int STAGE_ROWS = ROWS + COLS;                            // rows of 64 k: X, then A
-  static constexpr int RING_BYTES = kShrinkStages * STAGE_ROWS * 128;       // per warp
+  static constexpr int ROWS = kShrinkFewRows, COLS = 8 * NT8, LD = COLS + 8;
+  static constexpr int STAGE_BYTES = (ROWS + COLS) * 128;                   // rows of 64 k: X, then A
+  static constexpr int RING_BYTES = 2 * STAGE_BYTES;                        // per warp
   static constexpr int SMEM_BYTES = kShrinkWarps * RING_BYTES + ROWS * COLS * 4;
   static_assert(ROWS * LD * 4 <= RING_BYTES, "a warp's sums take the place of its stages");
-  static_assert(SMEM_BYTES <= 231424, "shared memory budget");
 };
 
 __device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool in) {
@@ -143,13 +142,14 @@ __device__ __forceinline__ void shrink_finish(const ShrinkArgs& args, const Shri
   }
 }
 
+// 128-byte rows of a stage; sixteen-byte unit u of row r sits at unit u ^ shrink_swizzle(r): a read takes four units of
+// eight rows, and any two neighbouring rows then lie in different halves of the banks.
 __device__ __forceinline__ int shrink_swizzle(int row) { return (row & 1) << 2 | (row >> 1 & 3); }
 
-template <int MT, int NT8>
+template <int NT8>
 __global__ void __launch_bounds__(32 * kShrinkWarps)
 lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
-  using S = ShrinkShape<MT, NT8>;
-  constexpr int WORDS = (S::ROWS + 31) / 32;
+  using S = ShrinkShape<NT8>;
   extern __shared__ __align__(16) uint8_t shrink_smem[];
   float* block_sums = reinterpret_cast<float*>(shrink_smem + kShrinkWarps * S::RING_BYTES);   // [row][COLS]
   __shared__ int slot_of[S::ROWS], id_of[S::ROWS];
@@ -162,20 +162,14 @@ lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
   if (!args.beside) pdl_wait();
   pdl_launch_dependents();
 
-  TileIds<WORDS> ids;
+  TileIds<1> ids;
   ids.load(args.ids, row0, row_end, lane);
-  if (warp == 0) {
-#pragma unroll
-    for (int w = 0; w < WORDS; ++w)
-      if (32 * w + lane < S::ROWS) id_of[32 * w + lane] = ids.id[w];
-  }
+  if (warp == 0 && lane < S::ROWS) id_of[lane] = ids.id[0];
   int slots = 0;
   while (ids.next() >= 0) ++slots;
   ids.last = -1;
-  const int by_slot = slots > 4 ? 8 : slots > 2 ? 4 : slots > 1 ? 2 : 1;
-  const int by_k = kShrinkWarps / by_slot;
-  const int my_slot = warp % by_slot;
-  // K: a run of steps per block, which its warps take in turn (together they read a row 1 KB at a time)
+  const int by_slot = slots > 2 ? 4 : slots > 1 ? 2 : 1, by_k = kShrinkWarps / by_slot;
+  // K: a run of steps per block, which the warps of an adapter take in turn
   const int steps = (pr.K + kShrinkK - 1) / kShrinkK, per = (steps + ranks - 1) / ranks;
   const int step0 = min(steps, rank * per) + warp / by_slot, step1 = min(steps, (rank + 1) * per);
   float* warp_sums = reinterpret_cast<float*>(shrink_smem + warp * S::RING_BYTES);            // [row][LD], once the stages are done
@@ -184,40 +178,29 @@ lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
 
   for (int slot = 0; slot < slots; ++slot) {
     const int a = ids.next();
-    if (slot % by_slot != my_slot) continue;
-    float acc[MT][NT8][4];
+    if (slot != warp % by_slot) continue;
+    float acc[NT8][2];   // rows g < 4 (the products' rows 4 to 7 repeat them, 8 to 15 are nothing)
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < NT8; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc[mt][nt][e] = a < args.n ? 0.f : NAN;
+    for (int nt = 0; nt < NT8; ++nt) acc[nt][0] = acc[nt][1] = 0.f;
     if (a < args.n) {
-      uint32_t wanted = 0;   // which of the rows cr, 4 + cr, ... this lane copies
-#pragma unroll
-      for (int i = 0; i < S::ROWS / 4; ++i)
-        wanted |= (__shfl_sync(0xffffffffu, ids.id[i / 8], (i * 4 + cr) % 32) == a ? 1u : 0u) << i;
+      const bool wanted = __shfl_sync(0xffffffffu, ids.id[0], cr) == a;   // whether this lane's row has the adapter
       const __nv_bfloat16* xp = pr.X + (int64_t)(row0 + cr) * pr.ldx + cc * 8;
       const __nv_bfloat16* ap = pr.A + (int64_t)a * pr.stride_a + (int64_t)(chunk * 64 + cr) * pr.lda + cc * 8;
       const int ranks_left = args.R - chunk * 64 - cr;
-      const int64_t x4 = 4 * pr.ldx, a4 = 4 * pr.lda;
+      const int64_t a4 = 4 * pr.lda;
       uint32_t dst_of[2];     // where this lane's copies of even and odd groups of four rows go in stage 0
 #pragma unroll
       for (int i = 0; i < 2; ++i) dst_of[i] = ring + (uint32_t)(cr * 128 + ((cc ^ shrink_swizzle(i * 4 + cr)) << 4));
-      // 128-byte rows; sixteen-byte unit u of row r sits at unit u ^ shrink_swizzle(r): a read takes four units of
-      // eight rows, and any two neighbouring rows then lie in different halves of the banks.  Rows of another adapter
-      // and ranks above R are not copied: what the stage holds there reaches only sums that nobody reads.
+      // Rows of another adapter and ranks above R are not copied: what the stage holds there reaches only sums that
+      // nobody reads.
       auto load = [&](int step, int stage) {   // one commit group per step, an empty one past the end
         if (step < step1) {
           const int k = step * kShrinkK;
           const bool in = k + cc * 8 < pr.K;   // K ends inside the step: zeros from there on
-          const uint32_t to = (uint32_t)(stage * S::STAGE_ROWS * 128);
-          const __nv_bfloat16* src = in ? xp + k : pr.X;
-          const int64_t dx = in ? x4 : 0, da = in ? a4 : 0;
-#pragma unroll
-          for (int i = 0; i < S::ROWS / 4; ++i, src += dx)
-            if (wanted >> i & 1u) cp_async_16(dst_of[i & 1] + to + i * 512, src, in);
-          src = in ? ap + k : pr.A;
+          const uint32_t to = (uint32_t)(stage * S::STAGE_BYTES);
+          if (wanted) cp_async_16(dst_of[0] + to, in ? xp + k : pr.X, in);
+          const __nv_bfloat16* src = in ? ap + k : pr.A;
+          const int64_t da = in ? a4 : 0;
 #pragma unroll
           for (int i = 0; i < S::COLS / 4; ++i, src += da)
             if (i * 4 < ranks_left) cp_async_16(dst_of[i & 1] + to + S::ROWS * 128 + i * 512, src, in);
@@ -230,68 +213,52 @@ lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
         load(step + by_k, stage ^ 1);   // into the stage that every lane is done with: the barrier at the end of the last round
         asm volatile("cp.async.wait_group 1;" ::: "memory");
         __syncwarp();
-        const uint32_t src = ring + (uint32_t)(stage * S::STAGE_ROWS * 128 + g * 128);
-        uint4 w[2][NT8];
-        const uint32_t unit[2] = {(uint32_t)(q ^ shrink_swizzle(g)) << 4, (uint32_t)((4 + q) ^ shrink_swizzle(g)) << 4};   // every row read is g mod 8
+        const uint32_t base = ring + (uint32_t)(stage * S::STAGE_BYTES);
+        uint4 x[2], w[2][NT8];
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int nt = 0; nt < NT8; ++nt) w[half][nt] = ld_shared_16(src + (S::ROWS + nt * 8) * 128 + unit[half]);
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          uint4 x[2][2];
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-#pragma unroll
-            for (int h = 0; h < 2; ++h) x[half][h] = ld_shared_16(src + mt * 2048 + h * 1024 + unit[half]);
-          // 64 k at a time in the tensor cores (which cut off low bits of a long running sum), added up in FP32
-          float t[NT8][4];
+        for (int half = 0; half < 2; ++half) {
+          x[half] = ld_shared_16(base + (g & 3) * 128 + (((half * 4 + q) ^ shrink_swizzle(g & 3)) << 4));
 #pragma unroll
           for (int nt = 0; nt < NT8; ++nt)
-            mma_m16n8k16_bf16_zero(t[nt], x[0][0].x, x[0][1].x, x[0][0].y, x[0][1].y, w[0][nt].x, w[0][nt].y);
+            w[half][nt] = ld_shared_16(base + (S::ROWS + nt * 8 + g) * 128 + (((half * 4 + q) ^ shrink_swizzle(g)) << 4));
+        }
+        // 64 k at a time in the tensor cores (which cut off low bits of a long running sum), added up in FP32
+        float t[NT8][4];
 #pragma unroll
-          for (int nt = 0; nt < NT8; ++nt) mma_m16n8k16_bf16(t[nt], x[0][0].z, x[0][1].z, x[0][0].w, x[0][1].w, w[0][nt].z, w[0][nt].w);
+        for (int nt = 0; nt < NT8; ++nt) mma_m16n8k16_bf16_zero(t[nt], x[0].x, 0u, x[0].y, 0u, w[0][nt].x, w[0][nt].y);
 #pragma unroll
-          for (int nt = 0; nt < NT8; ++nt) mma_m16n8k16_bf16(t[nt], x[1][0].x, x[1][1].x, x[1][0].y, x[1][1].y, w[1][nt].x, w[1][nt].y);
+        for (int nt = 0; nt < NT8; ++nt) mma_m16n8k16_bf16(t[nt], x[0].z, 0u, x[0].w, 0u, w[0][nt].z, w[0][nt].w);
 #pragma unroll
-          for (int nt = 0; nt < NT8; ++nt) mma_m16n8k16_bf16(t[nt], x[1][0].z, x[1][1].z, x[1][0].w, x[1][1].w, w[1][nt].z, w[1][nt].w);
+        for (int nt = 0; nt < NT8; ++nt) mma_m16n8k16_bf16(t[nt], x[1].x, 0u, x[1].y, 0u, w[1][nt].x, w[1][nt].y);
 #pragma unroll
-          for (int nt = 0; nt < NT8; ++nt)
+        for (int nt = 0; nt < NT8; ++nt) mma_m16n8k16_bf16(t[nt], x[1].z, 0u, x[1].w, 0u, w[1][nt].z, w[1][nt].w);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[mt][nt][e] += t[nt][e];
+        for (int nt = 0; nt < NT8; ++nt) {
+          acc[nt][0] += t[nt][0];
+          acc[nt][1] += t[nt][1];
         }
         __syncwarp();
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
       __syncwarp();
     }
-    float* sums = slots <= kShrinkWarps ? warp_sums : block_sums;
-    const int ld = slots <= kShrinkWarps ? S::LD : S::COLS;
+    const bool mine = __shfl_sync(0xffffffffu, ids.id[0], g) == a;
+    if (g < S::ROWS && mine) {
+      if (q == 0) slot_of[g] = slot;   // the same value from every warp that writes it
+      float* dst = warp_sums + g * S::LD + 2 * q;
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int lr = mt * 16 + h * 8 + g;
-        if (__shfl_sync(0xffffffffu, ids.id[(mt * 16 + h * 8) / 32], lr % 32) == a) {
-          if (q == 0) slot_of[lr] = slot;   // the same value from every warp that writes it
-          float* dst = sums + lr * ld + 2 * q;
-#pragma unroll
-          for (int nt = 0; nt < NT8; ++nt)
-            *reinterpret_cast<float2*>(dst + nt * 8) = make_float2(acc[mt][nt][2 * h], acc[mt][nt][2 * h + 1]);
-        }
-      }
+      for (int nt = 0; nt < NT8; ++nt) *reinterpret_cast<float2*>(dst + nt * 8) = make_float2(acc[nt][0], acc[nt][1]);
+    }
   }
   __syncthreads();
   const int elems = (row_end - row0) * S::COLS;
-  if (slots <= kShrinkWarps) {
-    for (int e = threadIdx.x; e < elems; e += 32 * kShrinkWarps) {
-      const int lr = e / S::COLS, c = e % S::COLS;
-      if (id_of[lr] < 0) continue;
-      float sum = 0.f;
-      for (int w = slot_of[lr] % by_slot; w < kShrinkWarps; w += by_slot)
-        sum += reinterpret_cast<const float*>(shrink_smem + w * S::RING_BYTES)[lr * S::LD + c];
-      block_sums[e] = sum;
-    }
+  for (int e = threadIdx.x; e < elems; e += 32 * kShrinkWarps) {
+    const int lr = e / S::COLS, c = e % S::COLS;
+    if (id_of[lr] < 0) continue;
+    float sum = 0.f;
+    for (int w = slot_of[lr]; w < kShrinkWarps; w += by_slot)
+      sum += reinterpret_cast<const float*>(shrink_smem + w * S::RING_BYTES)[lr * S::LD + c];
+    block_sums[e] = sum;
   }
   __syncthreads();
   shrink_finish<S::COLS>(args, pr, chunk, block_sums, id_of, row0, elems);
@@ -301,7 +268,7 @@ lora_shrink_kernel(const __grid_constant__ ShrinkArgs args) {
 // its own, X tiles (all rows of the block) and A tiles (one adapter each); one lane asks for another tile once
 // the oldest one has been multiplied, so a step costs the warp its reads from shared memory and
 // its products.  (With the copies of the kernel above, addresses and predicates were half of the instructions: 8192 x
-// 8192, one adapter per 512 rows, 41 us; now REPLACE_ROWS.)  The adapters of a block share the X tile, each multiplies the
+// 8192, rank 16, one adapter per 512 rows, 41 us; now 33, 4.1 TB/s.)  The adapters of a block share the X tile, each multiplies the
 // groups of 16 rows that have it, and a row takes up the products of its own adapter only: by selection, so that
 // nothing of another one reaches it.  Bound by the read of X where the rows of a request lie together.
 struct ShrinkMaps {

@@ -33,7 +33,7 @@ __device__ __forceinline__ void xent_merge(float& m, float& s, float pm, float p
 // Joins the column groups of every row, always in the same order.  A block of 1024 threads owns ROWS rows: thread
 // (slice, row) takes every 1024 / ROWS-th group, eight loads at a time.  With many rows 32 of them read 256 bytes of a group
 // together; with few, the threads go along the vocabulary instead (one row of 131072 columns as one slice
-// of 16 took 14 us, as 1024 slices REPLACE_FINISH).  Bound by the read of 8 T ceil(V / 128) bytes, 1/32 of
+// of 16 took 14 us, as 1024 slices 5 us).  Bound by the read of 8 T ceil(V / 128) bytes, 1/32 of
 // a bf16 copy of the logits.
 constexpr int kXentFinishThreads = 1024;
 template <int ROWS>
