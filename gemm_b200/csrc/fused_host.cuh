@@ -122,7 +122,8 @@ static int xent_sizes(const char* who, int64_t T, int64_t V, int64_t D, int64_t 
   if (T < 0 || V < 1 || D < 1) return fail(GEMM_B200_ERR_INVALID_ARG, "%s: T must not be negative, V and D must be positive", who);
   if (ldx < D || ldw < D)
     return fail(GEMM_B200_ERR_INVALID_ARG, "%s: leading dimension smaller than the row (ldx=%lld ldw=%lld)", who, (long long)ldx, (long long)ldw);
-  if (T > 0x7fffffff || V > 0x7fffff00 || D > 0x7fffffff) return fail(GEMM_B200_ERR_TOO_LARGE, "%s: a dimension exceeds 2^31-1", who);
+  // columns of the last tile and of the epilogue's look-ahead stay within 31 bits
+  if (T > 0x7fffffff || V > 0x7ffffc00 || D > 0x7fffffff) return fail(GEMM_B200_ERR_TOO_LARGE, "%s: a dimension exceeds 2^31-1", who);
   return GEMM_B200_OK;
 }
 
@@ -528,9 +529,9 @@ struct LoraGradScratch {
     v = c.take<__nv_bfloat16>(T * terms * lora_rp(R));
     perm = c.take<int32_t>(T);
     start = c.take<int32_t>(n + 1);
-    const bool parts = p.blocks > 1;
-    part_a = c.take<float>(parts ? (p.blocks + n) * R * D : 0);
-    part_b = c.take<float>(parts ? (p.blocks + n) * R * N : 0);
+    const int64_t parts = p.blocks > 1 ? 2 * p.blocks : 0;   // each block's first and last sum may be partial
+    part_a = c.take<float>(parts * R * D);
+    part_b = c.take<float>(parts * R * N);
     bytes = c.used;
   }
 };

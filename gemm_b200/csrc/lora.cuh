@@ -483,16 +483,16 @@ lora_sort_kernel(const int32_t* __restrict__ ids, int T, int n, int32_t* __restr
 // The token axis, sorted by adapter, is cut into blocks of equal length whatever the requests' shares are (one
 // adapter with every token, or sixty with a few each); a block owns 128 columns and walks the adapters that
 // its range touches, 32 tokens per step, the loads running ahead across the adapters' borders.
-// A sum that lies inside one block goes straight to the result; the others leave a partial sum at slot
-// (block + adapter), which no other pair shares because both only grow along the axis, and
-// lora_join_kernel adds them in the order of the blocks.  Rows are gathered, so only a request's own tokens
+// A sum that lies inside one block goes straight to the result.  The others, of which a block has two at
+// most, leave partial sums: in slot 2 b of block b the one that began in an earlier block, in slot 2 b + 1 the one
+// that begins there and goes on; lora_join_kernel adds them in the order of the blocks.  Rows are gathered, so only a request's own tokens
 // are ever multiplied: nothing of one request reaches another's gradient.
 // ---------------------------------------------------------------------------------------
 struct GradProblem {
   const __nv_bfloat16* P;   // [T, terms * rp]
   const __nv_bfloat16* Q;   // [T, cols], pitch ldq
   void* out;                // [n, R, cols]
-  float* part;              // [blocks + n][R][cols]
+  float* part;              // [2 * blocks][R][cols]
   int64_t ldq;
   int cols, first_chunk;    // column chunks [first_chunk, ...) of the grid belong to this problem
 };
@@ -660,6 +660,7 @@ lora_grad_kernel(const __grid_constant__ GradArgs args) {
     if (cu.pos >= cu.end) {   // the adapter's share of this block is complete
       const int a = cu.a;
       const bool whole = args.start[a] >= lo && args.start[a + 1] <= hi;
+      const int part_slot = 2 * (int)blockIdx.y + (args.start[a] >= lo ? 1 : 0);
       const long long out_elems = (long long)args.n * args.R * pr.cols;
       (void)out_elems;
 #pragma unroll
@@ -674,7 +675,7 @@ lora_grad_kernel(const __grid_constant__ GradArgs args) {
             if (c >= pr.cols) continue;
             const float x = acc[mt][nt][2 * h], y = acc[mt][nt][2 * h + 1];
             if (!whole) {
-              *reinterpret_cast<float2*>(pr.part + ((int64_t)(blockIdx.y + a) * args.R + r) * pr.cols + c) = make_float2(x, y);
+              *reinterpret_cast<float2*>(pr.part + ((int64_t)part_slot * args.R + r) * pr.cols + c) = make_float2(x, y);
             } else {
               const int64_t at = ((int64_t)a * args.R + r) * pr.cols + c;
               if (!GEMM_B200_IN_BOUNDS(static_cast<char*>(pr.out) + at * (OUT_F32 ? 4 : 2), pr.out, out_elems * (OUT_F32 ? 4 : 2), OUT_F32 ? 8 : 4, 51)) continue;
@@ -709,7 +710,7 @@ lora_join_kernel(const __grid_constant__ GradArgs args) {
     if (s1 > s0) {
 #pragma unroll 4
       for (int b = b0; b <= b1; ++b) {
-        const float4 v = *reinterpret_cast<const float4*>(pr.part + (int64_t)(b + a) * elems + e);
+        const float4 v = *reinterpret_cast<const float4*>(pr.part + (int64_t)(2 * b + (b == b0 ? 1 : 0)) * elems + e);
         acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
       }
     }

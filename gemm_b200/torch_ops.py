@@ -10,6 +10,10 @@ call them as opaque ops:
     aq, asf = torch.ops.gemm_b200.quantize_mxfp8(A)           # e4m3 bytes [M, K] + packed UE8M0 scales
     bq, bsf = torch.ops.gemm_b200.quantize_mxfp8(B, True)     # B given as [K, N]
     C = torch.ops.gemm_b200.gemm_mxfp8(aq, asf, bq, bsf)
+    loss, lse = torch.ops.gemm_b200.gemm_bf16_xent(X, W, labels)                    # vocabulary projection W [V, D]
+    dX, dW = torch.ops.gemm_b200.gemm_bf16_xent_grad(X, W, labels, lse, grad_loss)
+    Y = torch.ops.gemm_b200.gemm_bf16_lora(X, W, A, B, ids, scales, b_is_nk=True)   # adapters A [n, R, D], B [n, R, N]
+    dA, dB = torch.ops.gemm_b200.gemm_bf16_lora_grad(X, dY, A, B, ids, scales)
 
 The allocating forms are registered (out-parameter forms alias their argument, which the
 reference's wrappers do by design, naive/naive.cpp:17-21, and which functional graphs cannot
@@ -110,3 +114,53 @@ def gemm_mxfp8(a_data: torch.Tensor, a_scales: torch.Tensor, b_data: torch.Tenso
 def _(a_data, a_scales, b_data, b_scales, out_f32=False):
     torch._check(a_data.dim() == 2 and b_data.dim() == 2 and a_data.shape[1] == b_data.shape[1])
     return a_data.new_empty((a_data.shape[0], b_data.shape[0]), dtype=torch.float32 if out_f32 else torch.bfloat16)
+
+
+# Vocabulary loss and adapters of many requests; the gradients are operators of their own.
+@torch.library.custom_op("gemm_b200::gemm_bf16_xent", mutates_args=())
+def gemm_bf16_xent(X: torch.Tensor, W: torch.Tensor, labels: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    return ops.gemm_bf16_xent(X, W, labels)
+
+
+@gemm_bf16_xent.register_fake
+def _(X, W, labels):
+    torch._check(X.dim() == 2 and W.dim() == 2 and X.shape[1] == W.shape[1] and labels.dim() == 1)
+    return X.new_empty((X.shape[0],), dtype=torch.float32), X.new_empty((X.shape[0],), dtype=torch.float32)
+
+
+@torch.library.custom_op("gemm_b200::gemm_bf16_xent_grad", mutates_args=())
+def gemm_bf16_xent_grad(X: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, lse: torch.Tensor, grad_loss: torch.Tensor,
+                        grad_lse: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    return ops.gemm_bf16_xent_grad(X, W, labels, lse, grad_loss, grad_lse)
+
+
+@gemm_bf16_xent_grad.register_fake
+def _(X, W, labels, lse, grad_loss, grad_lse=None):
+    torch._check(X.dim() == 2 and W.dim() == 2 and X.shape[1] == W.shape[1])
+    return X.new_empty(X.shape), W.new_empty(W.shape)
+
+
+@torch.library.custom_op("gemm_b200::gemm_bf16_lora", mutates_args=())
+def gemm_bf16_lora(X: torch.Tensor, W: torch.Tensor, A: torch.Tensor, B: torch.Tensor, ids: torch.Tensor,
+                   scales: torch.Tensor | None = None, b_is_nk: bool = False, out_f32: bool = False) -> torch.Tensor:
+    return ops.gemm_bf16_lora(X, W, A, B, ids, scales, b_is_nk=b_is_nk, out_dtype=torch.float32 if out_f32 else torch.bfloat16)
+
+
+@gemm_bf16_lora.register_fake
+def _(X, W, A, B, ids, scales=None, b_is_nk=False, out_f32=False):
+    torch._check(X.dim() == 2 and W.dim() == 2 and A.dim() == 3 and B.dim() == 3)
+    n = W.shape[0] if b_is_nk else W.shape[1]
+    return X.new_empty((X.shape[0], n), dtype=torch.float32 if out_f32 else torch.bfloat16)
+
+
+@torch.library.custom_op("gemm_b200::gemm_bf16_lora_grad", mutates_args=())
+def gemm_bf16_lora_grad(X: torch.Tensor, dY: torch.Tensor, A: torch.Tensor, B: torch.Tensor, ids: torch.Tensor,
+                        scales: torch.Tensor | None = None, out_f32: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    return ops.gemm_bf16_lora_grad(X, dY, A, B, ids, scales, out_dtype=torch.float32 if out_f32 else torch.bfloat16)
+
+
+@gemm_bf16_lora_grad.register_fake
+def _(X, dY, A, B, ids, scales=None, out_f32=False):
+    torch._check(X.dim() == 2 and dY.dim() == 2 and A.dim() == 3 and B.dim() == 3)
+    dt = torch.float32 if out_f32 else torch.bfloat16
+    return A.new_empty(A.shape, dtype=dt), B.new_empty(B.shape, dtype=dt)
