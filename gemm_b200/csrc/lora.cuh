@@ -675,7 +675,8 @@ lora_grad_kernel(const __grid_constant__ GradArgs args) {
             if (c >= pr.cols) continue;
             const float x = acc[mt][nt][2 * h], y = acc[mt][nt][2 * h + 1];
             if (!whole) {
-              *reinterpret_cast<float2*>(pr.part + ((int64_t)part_slot * args.R + r) * pr.cols + c) = make_float2(x, y);
+              float* dst = pr.part + ((int64_t)part_slot * args.R + r) * pr.cols + c;
+              if (GEMM_B200_IN_BOUNDS(dst, pr.part, 2ll * args.blocks * args.R * pr.cols * 4, 8, 52)) *reinterpret_cast<float2*>(dst) = make_float2(x, y);
             } else {
               const int64_t at = ((int64_t)a * args.R + r) * pr.cols + c;
               if (!GEMM_B200_IN_BOUNDS(static_cast<char*>(pr.out) + at * (OUT_F32 ? 4 : 2), pr.out, out_elems * (OUT_F32 ? 4 : 2), OUT_F32 ? 8 : 4, 51)) continue;
@@ -715,6 +716,7 @@ lora_join_kernel(const __grid_constant__ GradArgs args) {
       }
     }
     const int64_t at = (int64_t)a * elems + e;
+    if (!GEMM_B200_IN_BOUNDS(static_cast<char*>(pr.out) + at * (OUT_F32 ? 4 : 2), pr.out, (long long)args.n * elems * (OUT_F32 ? 4 : 2), OUT_F32 ? 16 : 8, 53)) continue;
     if constexpr (OUT_F32) {
       *reinterpret_cast<float4*>(static_cast<float*>(pr.out) + at) = acc;
     } else {

@@ -84,6 +84,7 @@ xent_finish_kernel(const float2* __restrict__ part, const float* __restrict__ la
   const int out = blockIdx.x * ROWS + warp;
   if (lane != 0 || out >= T) return;
   const float total = (isinf(m) ? 0.f : m) + logf(s);
+  if (!GEMM_B200_IN_BOUNDS(lse + out, lse, (long long)T * 4, 4, 42)) return;
   const int64_t label = labels[out];
   lse[out] = total;
   loss[out] = label < 0 ? 0.f : (label >= V ? NAN : total - label_logit[out]);

@@ -196,6 +196,7 @@ size_t gemm_b200_gemm_bf16_xent_scratch_bytes(int64_t T, int64_t V);
  * negative), h = grad_lse (likewise; NULL = 0).  A stride of 0 is a scalar.  The logits are recomputed a
  * piece of the vocabulary at a time; d is rounded to bf16 between the products.  A row with g = h = 0
  * adds nothing to dW whatever X holds there; a label >= V makes its row of dX, and dW, NaN.
+ * d is kept as two bf16 summands for T <= 64.
  * The outputs may not overlap the inputs or each other.  Requirements: as above, also for dX and dW;
  * D a multiple of 8.  The scratch size is for the current device. */
 int gemm_b200_gemm_bf16_xent_grad(const void* X, const void* W, const int64_t* labels, const float* lse,
@@ -217,7 +218,7 @@ size_t gemm_b200_gemm_bf16_xent_grad_scratch_bytes(int64_t T, int64_t V, int64_t
  * exchanged.  The reference has no counterpart; the product extends its operator
  * (naive/naive.cpp:6-22).
  * Requirements: pointers 16-byte aligned; D, N, every leading dimension and stride multiples of 8 (ldy * sizeof(Y)
- * of 16 bytes); scratch as above.
+ * of 16 bytes); Y overlaps no input; scratch as above.
  * ------------------------------------------------------------------------- */
 int gemm_b200_gemm_bf16_lora(const void* X, const void* W, const void* A, const void* B, const int32_t* ids,
                              const float* scales, void* Y, int64_t T, int64_t N, int64_t D, int64_t R, int64_t adapters,
