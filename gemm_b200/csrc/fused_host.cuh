@@ -127,8 +127,9 @@ static int xent_sizes(const char* who, int64_t T, int64_t V, int64_t D, int64_t 
   return GEMM_B200_OK;
 }
 
-// The gradient works on pieces of the vocabulary whose d (bf16) takes at most this much scratch.
-constexpr int64_t kXentPieceBytes = 256ll << 20;
+// The gradient works on pieces of the vocabulary whose d (bf16) takes at most this much scratch, but of 4096 columns at
+// least: every piece but the first adds T x D FP32 values to dX, which a shorter product would not hide.
+constexpr int64_t kXentPieceBytes = 256ll << 20, kXentMinPiece = 4096;
 
 struct XentGradPlan {
   int halves;                 // bf16 summands of d, one below the other: two for up to 64 rows, one row tile (xent.cuh)
@@ -139,7 +140,7 @@ struct XentGradPlan {
     halves = 2 * T <= kBlockM ? 2 : 1;
     const int64_t rows = halves * T;
     int64_t most = kXentPieceBytes / (2 * (rows > 0 ? rows : 1)) / kBlockN * kBlockN;
-    if (most < 2 * kBlockN) most = 2 * kBlockN;
+    if (most < kXentMinPiece) most = kXentMinPiece;
     pieces = ceil_div64(V, most);
     piece = pieces == 1 ? V : ceil_div64(ceil_div64(V, pieces), kBlockN) * kBlockN;
     pieces = ceil_div64(V, piece);

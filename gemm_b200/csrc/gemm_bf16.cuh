@@ -252,7 +252,7 @@ struct XentGradFuse {
 // operand would.
 struct LoraFuse {
   static constexpr FuseKind KIND = kFuseLora;
-  CUtensorMap tmV;          // [M, terms * rp], box 64 x 128
+  CUtensorMap tmV;          // [M, terms * rp], the box of A's tiles
   CUtensorMap tmAd;         // [adapters][R][N], box 64 columns x min(rp, 64) rows; ranks above R read as zero
   const int32_t* ids;       // [M]
   int rp, terms;

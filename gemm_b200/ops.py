@@ -332,7 +332,7 @@ def gemm_bf16_xent_grad(X: torch.Tensor, W: torch.Tensor, labels: torch.Tensor, 
 
     ``grad_loss`` (and ``grad_lse``, for a loss that uses the log-sum-exp too) are FP32 ``[T]`` of any stride, so
     the expanded scalar that a sum's gradient is goes in as it is.  The logits are recomputed a piece of the
-    vocabulary at a time.  A row whose gradients are zero, as padding's are, adds nothing to ``dW`` whatever
+    vocabulary at a time.  D must be a multiple of 8.  A row whose gradients are zero, as padding's are, adds nothing to ``dW`` whatever
     its ``X`` holds.  ``grad_loss`` is not read where the label is negative; a label >= V makes its
     row of ``dX``, and ``dW``, NaN."""
     device, T, V, D, ldx, ldw = _xent_operands(X, W, labels)

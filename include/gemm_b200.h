@@ -213,7 +213,8 @@ size_t gemm_b200_gemm_bf16_xent_grad_scratch_bytes(int64_t T, int64_t V, int64_t
  * B_a = B + a * stride_b, [R,N] with pitch ldb; ids int32 [T] on the device, in any order; scales FP32
  * [adapters] on the device (NULL = 1).  A negative id means no adapter, an id >= adapters makes its row
  * NaN.  Infinities and NaN in one adapter reach only the rows that use it.  R <= 128.
- * X A^T is kept as one bf16 value for bf16 output and as three summands (24 bits) for FP32 output.
+ * X A^T is kept as three bf16 summands (24 bits) for FP32 output and for at most 64 rows at a rank of at
+ * most 16, and as one bf16 value otherwise.
  * The gradient with respect to X is the same call with dY for X, W in the other layout, and A and B
  * exchanged.  The reference has no counterpart; the product extends its operator
  * (naive/naive.cpp:6-22).

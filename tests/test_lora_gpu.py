@@ -82,7 +82,8 @@ def check(ops, X, W, A, B, ids, s, nk, f32):
 @pytest.mark.parametrize("T,N,D,R,n,order", [
     (1, 8, 8, 1, 1, "one"), (1, 512, 264, 16, 4, "one"), (2, 200, 64, 8, 3, "mixed"), (17, 264, 136, 17, 5, "mixed"), (64, 256, 512, 16, 64, "mixed"),
     (65, 1032, 200, 33, 70, "mixed"), (128, 128, 128, 64, 128, "mixed"), (129, 520, 256, 100, 9, "sorted"), (257, 264, 72, 128, 300, "mixed"),
-    (300, 512, 256, 16, 40, "none"), (1030, 264, 520, 48, 7, "sorted"), (1100, 128, 1000, 16, 50, "mixed"), (1500, 776, 320, 32, 3, "one"),
+    (300, 512, 256, 16, 40, "none"), (511, 128, 264, 20, 60, "mixed"), (512, 128, 264, 20, 60, "mixed"), (600, 64, 8192, 16, 30, "mixed"),
+    (700, 136, 1032, 128, 40, "mixed"), (600, 72, 4104, 50, 30, "sorted"), (32, 264, 4096, 16, 20, "mixed"), (33, 520, 72, 8, 33, "mixed"), (1030, 264, 520, 48, 7, "sorted"), (1100, 128, 1000, 16, 50, "mixed"), (1500, 776, 320, 32, 3, "one"),
 ])
 def test_projection_with_adapters(ops, T, N, D, R, n, order, nk, f32):
     check(ops, *make(T, N, D, R, n, order, nk, seed=T + R), nk, f32)

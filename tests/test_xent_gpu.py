@@ -75,6 +75,26 @@ def test_loss_and_gradient(ops, T, V, D):
     check(ops, *make(T, V, D, seed=T + V))
 
 
+@pytest.mark.parametrize("T", [16, 31, 32, 33, 64, 65, 128, 129])
+def test_around_the_row_counts_where_the_kernels_change(ops, T):
+    """32, 64, 128 rows: the box of X; up to 64 rows: d in two bf16 summands; above 128: CTA pairs."""
+    check(ops, *make(T, 2050, 264, seed=T))
+
+
+def test_few_rows_keep_more_of_d_than_one_bf16_value(ops):
+    # one row: with a single rounding of the label's entry dX could be off by 2^-8 of itself, now only by its own rounding
+    for seed in range(8):
+        X, W, lab, gl, _ = make(1, 3000, 256, seed=seed)
+        gl = gl.abs() + 0.1
+        _, lse = ops.gemm_bf16_xent(X, W, lab)
+        dX, dW = ops.gemm_bf16_xent_grad(X, W, lab, lse, gl)
+        want, _ = exact(X, W, lab, gl)
+        for got, w in ((dX, want[2]), (dW, want[3])):
+            off = (got.double() - w).abs()
+            # its own half step, two summands of d (2^-16) and the logits' and log-sum-exp's FP32 errors (below 2^-14)
+            assert (off <= HALF * w.abs() + 2.0 ** -13 * w.abs().max()).all()
+
+
 def test_gradient_through_the_log_sum_exp(ops):
     check(ops, *make(200, 777, 128)[:4], make(200, 777, 128)[4])
 
