@@ -86,7 +86,7 @@ def _headers() -> list[Path]:
 
 
 def build_library(force: bool = False, verbose: bool = False) -> Path:
-    BUILD.mkdir(exist_ok=True)
+    BUILD.mkdir(parents=True, exist_ok=True)
     hdrs = _headers()
     jobs = []
     objs = []
@@ -186,10 +186,11 @@ def build_variant(variant: str, force: bool = False) -> Path:
 
 
 def build_all(variants: bool = True, force: bool = False, verbose: bool = False) -> None:
-    build_library(force=force, verbose=verbose)
-    build_probe(force=force)
-    build_trace(force=force)
-    build_debug(force=force)
+    # the library and its diagnostic flavours compile the same sources independently: side by side
+    with cf.ThreadPoolExecutor(max_workers=4) as ex:
+        jobs = [ex.submit(build_library, force=force, verbose=verbose)] + [ex.submit(f, force=force) for f in (build_probe, build_trace, build_debug)]
+        for j in jobs:
+            j.result()
     if variants:
         with cf.ThreadPoolExecutor(max_workers=3) as ex:
             list(ex.map(lambda v: build_variant(v, force=force), VARIANTS))
